@@ -1,0 +1,73 @@
+// Attention of packed whole prompts: causal self-attention of the tokens of
+// each sequence, grouped heads, contiguous 16-bit q, k and v.  The kernel is
+// rows_kernel of attention_rows.hpp.
+#include "attention_rows.hpp"
+
+namespace fellm {
+namespace {
+using namespace rows_attn;
+
+template <typename E, int HD, int RW, int KW, int KT, int OCC>
+int launch_prompt(Args a, hipStream_t st) {
+    constexpr uint32_t BM = kRows * RW;
+    const uint64_t tiles = (uint64_t)a.tokens * a.group / BM + a.n_seqs;
+    if (tiles * a.n_kv > 0xffffffffull / (kWave * RW * KW)) return FELLM_ERR_SHAPE;
+    FELLM_LAUNCH((rows_kernel<E, HD, RW, KW, KT, false, false, OCC>), dim3((uint32_t)tiles * a.n_kv),
+                 dim3(kWave * RW * KW), 0, st, a);
+    return launch_status();
+}
+
+template <typename E>
+int prompt_heads(uint32_t head_dim, const Args &a, hipStream_t st) {
+    if (head_dim == 64) return launch_prompt<E, 64, 4, 1, 64, 2>(a, st);
+    if (head_dim == 128) return launch_prompt<E, 128, 4, 1, 64, 2>(a, st);
+    if (head_dim == 256) return launch_prompt<E, 256, 4, 1, 32, 1>(a, st);
+    return FELLM_ERR_SHAPE;
+}
+
+}  // namespace
+}  // namespace fellm
+
+extern "C" int fellm_rocm_prompt_attention(const void *q, uint32_t q_stride, const void *k, uint32_t k_stride,
+                                           const void *v, uint32_t v_stride, void *out, uint32_t dtype,
+                                           const uint32_t *cu_seqlens, uint32_t n_seqs, uint32_t tokens,
+                                           uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, float scale,
+                                           uint32_t causal, uint32_t window, void *stream) {
+    using namespace fellm;
+    if (dtype != FELLM_DTYPE_F16 && dtype != FELLM_DTYPE_BF16) return FELLM_ERR_DTYPE;
+    if (!n_kv_heads || !n_heads || n_heads % n_kv_heads) return FELLM_ERR_SHAPE;
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) return FELLM_ERR_SHAPE;
+    if (n_seqs == 0 || tokens == 0) return FELLM_OK;
+    if (!q || !k || !v || !out || !cu_seqlens) return FELLM_ERR_ARITY;
+    const uint64_t qw = (uint64_t)n_heads * head_dim, kw = (uint64_t)n_kv_heads * head_dim;
+    if (qw > 0x7fffffffull || (uint64_t)tokens * n_heads > 0x7fffffffull) return FELLM_ERR_SHAPE;
+    if (q_stride < qw || k_stride < kw || v_stride < kw) return FELLM_ERR_SHAPE;
+    // 16-byte pieces, and 16 rows of a tile inside a buffer resource's 31 bits
+    if (q_stride % 8 || k_stride % 8 || v_stride % 8 || k_stride > (1u << 26) || v_stride > (1u << 26)) return FELLM_ERR_SHAPE;
+    if (!aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(out, 16)) return FELLM_ERR_SHAPE;
+    if (!(scale > 0.0f)) scale = 1.0f / sqrtf((float)head_dim);
+    rows_attn::Args a{};
+    a.q = q;
+    a.out = out;
+    a.k = static_cast<const uint8_t *>(k);
+    a.v = static_cast<const uint8_t *>(v);
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.out_stride = (uint32_t)qw;
+    a.q_dtype = a.out_dtype = dtype;
+    a.cu = cu_seqlens;
+    a.n_seqs = n_seqs;
+    a.tokens = tokens;
+    a.n_heads = n_heads;
+    a.n_kv = n_kv_heads;
+    a.group = n_heads / n_kv_heads;
+    a.c = scale * 1.4426950408889634f;
+    a.causal = causal;
+    a.window = window;
+    a.splits = 1;
+    a.keys_per_split = 0x7fffffc0u;
+    hipStream_t st = as_stream(stream);
+    return dtype == FELLM_DTYPE_BF16 ? prompt_heads<rows_attn::ElemBF16>(head_dim, a, st)
+                                     : prompt_heads<rows_attn::ElemF16>(head_dim, a, st);
+}

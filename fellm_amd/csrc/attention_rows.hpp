@@ -1,0 +1,639 @@
+// Attention of several query rows per sequence on the matrix cores: the body
+// shared by prompt attention (contiguous K/V, attention_prompt.hip) and tree
+// attention (paged K/V, attention_tree.hip).
+//
+// Mathematics.  A row is one (token i, query head) pair; the G = n_heads /
+// n_kv heads that share a K/V head are packed, row r = i G + head, so that a
+// tile of rows reads every K/V byte once for all of them.  Per row, over its
+// attended keys j: s_j = q . k_j, p_j = exp2(c (s_j - m)) with c = scale log2 e,
+// out = sum p_j v_j / sum p_j, the maximum m and the sum running in f32.
+//
+// Layout.  A wavefront owns 32 rows and walks tiles of KT keys staged in LDS:
+//  * S^T = K Q^T by v_mfma_f32_32x32x16: A = K (lane: key lane % 32, 8 dims),
+//    B = Q^T held in registers.  Lane (n, h) = (lane % 32, lane / 32) then has
+//    the scores of row n with keys 8 (i / 4) + 4 h + i % 4, i = 0..15: maximum
+//    and sum are lane-local up to one exchange between the halves.
+//  * O^T = V^T P^T: p is rounded to 16 bits where it is, in the B layout; the
+//    order of keys inside a contraction is free, so V^T is read in the order
+//    the scores came in, by ds_read_b64_tr_b16 (4 keys x 16 dims transposed
+//    per 16 lanes).  O^T has its row in the lane too: rescaling is per lane.
+//  * K and V go to LDS straight from memory (buffer loads with lds), double
+//    buffered, one barrier per tile; keys past the end are out of the
+//    resource's range and arrive as zeros.  The 16-byte pieces of a key row are
+//    permuted by a bijection of the key's low bits (swizzle) that spreads both
+//    the 16-key reads of K and the 4-key x 32-dim reads of V over all banks.
+//  * The running maximum is raised only when a row's new maximum exceeds it by
+//    more than kLazy (in log2): p stays below 2^kLazy, and most tiles skip the
+//    rescaling of O.
+// A masked score is -inf before the exp; a masked V that is not finite makes
+// 0 x inf = NaN in the product, so rows whose result is not finite (or whose
+// sum is zero) are computed again key by key, over their attended keys alone.
+#pragma once
+
+#include "common.hpp"
+
+namespace fellm {
+namespace rows_attn {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+using Rsrc = __amdgpu_buffer_rsrc_t;
+
+constexpr uint32_t kRows = 32;         // rows of a wavefront
+constexpr uint32_t kBlockTokens = 16;  // tokens of a cache block
+
+// K/V element policies.  kBias: log2 added to every exponent, so that small
+// probabilities stay normal f16 numbers; it cancels in out = O / l.
+struct ElemF16 {
+    using A = F16;
+    static constexpr int kQParts = 2, kPParts = 2;  // parts that hold f32 operands
+    static constexpr float kBias = 4.0f, kBiasParts = 15.0f;
+    __device__ static f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+    }
+    // Two values rounded to nearest even and packed; the remainders replace them.
+    __device__ static uint32_t part(float &x, float &y) {
+        typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+        const half2 h = {(_Float16)x, (_Float16)y};
+        x -= (float)h[0];
+        y -= (float)h[1];
+        return __builtin_bit_cast(uint32_t, h);
+    }
+};
+struct ElemBF16 {
+    using A = BF16;
+    static constexpr int kQParts = 3, kPParts = 3;
+    static constexpr float kBias = 0.0f, kBiasParts = 0.0f;
+    __device__ static f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    __device__ static uint32_t part(float &x, float &y) {
+        typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+        const bf2 h = {(__bf16)x, (__bf16)y};
+        const uint32_t u = __builtin_bit_cast(uint32_t, h);
+        x -= __uint_as_float(u << 16);
+        y -= __uint_as_float(u & 0xffff0000u);
+        return u;
+    }
+};
+
+struct Args {
+    const void *q;
+    void *out;
+    const uint8_t *k, *v;   // contiguous K/V, 16-bit elements
+    uint32_t k_stride, v_stride, q_stride, out_stride;  // elements per token row
+    uint32_t q_dtype, out_dtype;
+    const uint32_t *cu;     // [n_seqs + 1] first token of each sequence
+    const uint32_t *before; // [n_seqs] cached keys before a sequence's first token, or null
+    const uint32_t *mask;   // [tokens, mask_words] bits of the sequence's own tokens, or null
+    uint32_t mask_words, n_seqs, tokens, n_heads, n_kv, group;
+    float c;                // scale log2 e
+    uint32_t causal, window;
+    uint32_t max_before;    // bound that `before` is clamped to
+    // paged K/V
+    const uint8_t *arena;
+    uint64_t arena_len, block_bytes, n_table;
+    const uint32_t *table;
+    uint32_t n_logical, n_layers, layer, stride;
+    // split of the keys
+    uint32_t splits, keys_per_split;
+    float *part;
+};
+
+// A tile of rows: sequence, its tokens and the keys before them.
+struct Tile {
+    uint32_t seq, row0;      // first packed row inside the sequence
+    uint32_t first, n;       // first token in the packed tensors, tokens
+    uint32_t before;
+};
+
+// Tiles are numbered so that no prefix sum over the sequences is needed:
+// sequence b's first tile is floor(cu[b] G / BM) + b, which leaves room for its
+// ceil(n_b G / BM) tiles; numbers past a sequence's rows are empty.
+template <uint32_t BM>
+__device__ __forceinline__ Tile find_tile(const Args &a, uint32_t t) {
+    const uint32_t lane = threadIdx.x % kWave;
+    uint32_t lo = 0, len = a.n_seqs;
+    while (len > 1) {
+        const uint32_t step = (len + kWave - 1) / kWave, b = lane * step;
+        const bool le = b < len && min(a.cu[lo + min(b, len - 1)], a.tokens) * a.group / BM + lo + b <= t;
+        const uint32_t below = max(1u, (uint32_t)__popcll(__ballot(le)));
+        lo += (below - 1) * step;
+        len = min(step, len - (below - 1) * step);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    Tile r;
+    r.seq = lo;
+    r.first = min(a.cu[lo], a.tokens);
+    const uint32_t end = min(a.cu[lo + 1], a.tokens);
+    r.n = end > r.first ? end - r.first : 0;
+    r.row0 = (t - (r.first * a.group / BM + lo)) * BM;
+    r.before = a.before ? min(a.before[lo], a.max_before) : 0;
+    if (r.row0 >= r.n * a.group) r.n = 0;
+    return r;
+}
+
+// Attended keys of token i: [lo, hi), all of them or, at and past `before`, those with a bit.
+struct KeyRange {
+    uint32_t lo, hi;
+};
+__device__ __forceinline__ KeyRange row_keys(const Args &a, const Tile &t, uint32_t i) {
+    const uint32_t all = t.before + t.n;
+    KeyRange r{0, all};
+    if (a.mask) return r;
+    if (a.causal) {
+        r.hi = t.before + i + 1;
+        if (a.window && r.hi > a.window) r.lo = r.hi - a.window;
+    } else if (a.window) {
+        r.lo = i >= a.window ? i - a.window + 1 : 0;
+        r.hi = a.window < all - i ? i + a.window : all;
+    }
+    return r;
+}
+
+// Bit b: key kb + b (b < 64) is attended by the row.
+__device__ __forceinline__ uint64_t key_bits(const Args &a, const Tile &t, uint32_t token, KeyRange r, uint32_t kb) {
+    auto below = [&](uint32_t end) -> uint64_t {  // bits of keys < end
+        const uint32_t n = end > kb ? end - kb : 0;
+        return n >= 64 ? ~0ull : (1ull << n) - 1;
+    };
+    uint64_t bits = below(r.hi) & ~below(r.lo);
+    if (a.mask && kb + 64 > t.before) {
+        const uint64_t prefix = below(t.before);
+        // the 64 mask bits from own token kb - before on (negative: none yet)
+        const uint32_t *row = a.mask + (size_t)(t.first + token) * a.mask_words;
+        const int64_t at = (int64_t)kb - (int64_t)t.before;
+        const int32_t w = (int32_t)(at >> 5);
+        const uint32_t sh = (uint32_t)(at & 31);
+        uint32_t x[3];
+#pragma unroll
+        for (int e = 0; e < 3; ++e) x[e] = w + e >= 0 && (uint32_t)(w + e) < a.mask_words ? row[w + e] : 0;
+        const uint64_t lo = x[0] | (uint64_t)x[1] << 32;
+        const uint64_t own = sh ? lo >> sh | (uint64_t)x[2] << (64 - sh) : lo;
+        bits &= prefix | own;
+    }
+    return bits;
+}
+
+// Element pointers of key j (byte address), or null where the cache has no such block.
+template <bool PAGED>
+__device__ __forceinline__ const uint8_t *key_ptr(const Args &a, const Tile &t, uint32_t g, uint32_t hd, uint32_t j,
+                                                  bool is_v) {
+    if constexpr (PAGED) {
+        const uint32_t blk = j / kBlockTokens;
+        const size_t ti = ((size_t)t.seq * a.n_layers + a.layer) * a.n_logical + blk;
+        if (blk >= a.n_logical || ti >= a.n_table) return nullptr;
+        const uint64_t p = a.table[ti];
+        if ((p + 1) * a.block_bytes > a.arena_len) return nullptr;
+        return a.arena + p * a.block_bytes +
+               ((uint64_t)(j % kBlockTokens + (is_v ? kBlockTokens : 0)) * a.stride + (uint64_t)g * hd) * 2;
+    } else {
+        const uint32_t stride = is_v ? a.v_stride : a.k_stride;
+        return (is_v ? a.v : a.k) + ((size_t)(t.first + j) * stride + (size_t)g * hd) * 2;
+    }
+}
+
+__device__ __forceinline__ float load_elem(const void *p, uint32_t dtype, size_t i) {
+    if (dtype == FELLM_DTYPE_F32) return static_cast<const float *>(p)[i];
+    if (dtype == FELLM_DTYPE_F16) return F16::load(static_cast<const _Float16 *>(p)[i]);
+    return BF16::load(static_cast<const uint16_t *>(p)[i]);
+}
+__device__ __forceinline__ void store_elem(void *p, uint32_t dtype, size_t i, float v) {
+    if (dtype == FELLM_DTYPE_F32) static_cast<float *>(p)[i] = v;
+    else if (dtype == FELLM_DTYPE_F16) static_cast<_Float16 *>(p)[i] = F16::store(v);
+    else static_cast<uint16_t *>(p)[i] = BF16::store(v);
+}
+
+// One row over the keys [k0, k1), by one wavefront, key by key: only attended
+// keys are touched.  Unnormalised sums in acc (dims lane + 64 e), m, l, all
+// times 2^bias as the tiles' are.
+template <typename E, int HD, bool PAGED>
+__device__ void careful_row(const Args &a, const Tile &t, uint32_t g, uint32_t token, uint32_t head, uint32_t k0,
+                            uint32_t k1, float bias, float (&acc)[HD / 64], float &m, float &l) {
+    using T = typename E::A::T;
+    const uint32_t lane = threadIdx.x % kWave;
+    const KeyRange r = row_keys(a, t, token);
+    const size_t q0 = (size_t)(t.first + token) * a.q_stride + (size_t)head * HD;
+    auto score = [&](uint32_t j) -> float {
+        const T *kp = reinterpret_cast<const T *>(key_ptr<PAGED>(a, t, g, HD, j, false));
+        float s = 0.0f;
+#pragma unroll 1
+        for (int d = 0; d < HD; ++d) s = fmaf(load_elem(a.q, a.q_dtype, q0 + d), kp ? E::A::load(kp[d]) : 0.0f, s);
+        return s;
+    };
+    auto attended = [&](uint32_t kb) -> uint64_t {
+        const uint64_t bits = key_bits(a, t, token, r, kb);
+        return kb + 64 > k1 ? bits & ((1ull << (k1 - kb)) - 1) : bits;
+    };
+    m = -__builtin_inff();
+    l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < HD / 64; ++e) acc[e] = 0.0f;
+    for (uint32_t kb = k0; kb < k1; kb += 64) {
+        const uint64_t bits = attended(kb);
+        if (bits >> lane & 1) {
+            const float s = score(kb + lane);
+            m = s > m || s != s ? s : m;
+        }
+    }
+    float top = m;
+    bool nan = m != m;
+#pragma unroll
+    for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    m = __any(nan) ? __builtin_nanf("") : top;
+    for (uint32_t kb = k0; kb < k1; kb += 64) {
+        uint64_t bits = attended(kb);
+        if (!bits) continue;
+        const float p = bits >> lane & 1 ? __builtin_amdgcn_exp2f((score(kb + lane) - m) * a.c + bias) : 0.0f;
+        l += p;
+        while (bits) {
+            const uint32_t b = (uint32_t)__builtin_ctzll(bits);
+            bits &= bits - 1;
+            const float pb = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), b));
+            const T *vp = reinterpret_cast<const T *>(key_ptr<PAGED>(a, t, g, HD, kb + b, true));
+#pragma unroll
+            for (int e = 0; e < HD / 64; ++e) acc[e] = fmaf(pb, vp ? E::A::load(vp[lane + 64 * e]) : 0.0f, acc[e]);
+        }
+    }
+    l = wave_sum(l);
+}
+
+// The bijection of a key's low four (HD 64: bits 1 to 3) bits that its 16-byte
+// pieces are permuted by.
+template <int HD>
+__device__ __forceinline__ uint32_t swizzle(uint32_t key) {
+    if constexpr (HD == 64) return (key >> 1 & 1) << 2 | (key >> 2 & 1) << 1 | (key >> 3 & 1);
+    return (key & 3) << 2 | (key >> 2 & 1) << 1 | (key >> 3 & 1);
+}
+
+__device__ __forceinline__ float halves_max(float v) {
+    const uint32_t u = __float_as_uint(v);
+    const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+    const uint32_t u = __float_as_uint(v);
+    const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// A split's partial record of one row: HD unnormalised sums, m, l, two unused.
+template <int HD>
+constexpr uint32_t kRec = HD + 4;
+
+// Keys of a tile of rows, and the part of them that split z has.
+struct Share {
+    uint32_t begin, end;  // first a multiple of 64
+    uint32_t live;        // splits with keys (0: no keys at all)
+};
+template <uint32_t BM>
+__device__ __forceinline__ Share key_share(const Args &a, const Tile &t, uint32_t z) {
+    const uint32_t i0 = t.row0 / a.group, i1 = min(t.n, (t.row0 + BM - 1) / a.group + 1);
+    const KeyRange f = row_keys(a, t, i0), e = row_keys(a, t, i1 - 1);
+    uint32_t lo = f.lo / 64 * 64, hi = e.hi;
+    Share s;
+    const uint32_t total = hi > lo ? hi - lo : 0;
+    const uint32_t live = (total + a.keys_per_split - 1) / a.keys_per_split;
+    s.live = min(live, a.splits);
+    s.begin = lo + z * a.keys_per_split;
+    // the last split takes what is past the launch's bound on the keys
+    s.end = z + 1 >= s.live ? hi : min(hi, s.begin + a.keys_per_split);
+    return s;
+}
+
+// E: K/V policy, HD: head dim, RW: wavefronts that own 32 rows each, KW:
+// wavefronts that share those rows and take every KW-th key tile, KT: keys of
+// a wavefront's tile (32 or 64), PARTS: q and p held to f32 accuracy in several
+// 16-bit parts (q or out in f32, or q of another 16-bit type than K/V).
+template <typename E, int HD, int RW, int KW, int KT, bool PAGED, bool PARTS, int OCC>
+__global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
+    constexpr int NW = RW * KW, NS = HD / 16, NU = KT / 32, ND = HD / 32;
+    constexpr int QP = PARTS ? E::kQParts : 1, PP = PARTS ? E::kPParts : 1;
+    constexpr uint32_t BM = kRows * RW, TK = KT * KW, SK = TK / NW;  // keys a wavefront stages per round
+    constexpr uint32_t CH = HD / 8, RB = HD * 2;                      // 16-byte pieces, bytes of a key row
+    constexpr uint32_t KPI = kWave / CH;                              // keys per load instruction
+    constexpr float kBias = PARTS ? E::kBiasParts : E::kBias;
+    constexpr float kLazy = PARTS ? 0.0f : 8.0f;
+    static_assert(SK % KPI == 0 && (SK <= kBlockTokens || SK % kBlockTokens == 0) && 64 % SK == 0);
+    using T = typename E::A::T;
+
+    __shared__ __align__(16) uint8_t k_lds0[TK * RB], v_lds0[TK * RB], k_lds1[TK * RB], v_lds1[TK * RB];
+
+    const uint32_t lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t rw = wave % RW, kw = wave / RW;
+    const uint32_t n = lane % 32, h = lane / 32;
+    // Neighbouring workgroups take the K/V heads in turn (one XCD sees few of
+    // them), the tiles with most keys first.
+    const uint32_t per = gridDim.x / a.splits;
+    const uint32_t z = blockIdx.x / per, id = blockIdx.x % per;
+    const uint32_t g = id % a.n_kv, tiles = per / a.n_kv;
+    const uint32_t ti = tiles - 1 - id / a.n_kv;
+    const Tile t = find_tile<BM>(a, ti);
+    if (t.n == 0) return;
+    const Share sh = key_share<BM>(a, t, z);
+    if (z >= max(sh.live, 1u)) return;
+
+    const uint32_t row = t.row0 + rw * kRows + n;
+    const bool valid = row < t.n * a.group;
+    const uint32_t rrow = valid ? row : t.n * a.group - 1;
+    const uint32_t token = rrow / a.group, head = g * a.group + rrow % a.group;
+    const KeyRange mine = row_keys(a, t, token);
+    // keys that every row of this wavefront attends, and that any does
+    const uint32_t w0 = min(t.row0 + rw * kRows, t.n * a.group - 1), w1 = min(w0 + kRows - 1, t.n * a.group - 1);
+    const KeyRange rf = row_keys(a, t, w0 / a.group), rl = row_keys(a, t, w1 / a.group);
+    const uint32_t full_lo = rl.lo, full_hi = a.mask ? t.before : rf.hi, any_lo = rf.lo, any_hi = rl.hi;
+
+    u32x4 qf[NS][QP];
+    {
+        const size_t q0 = (size_t)(t.first + token) * a.q_stride + (size_t)head * HD + 8 * h;
+        if constexpr (!PARTS) {
+            const T *qp = static_cast<const T *>(a.q) + q0;
+#pragma unroll
+            for (int s = 0; s < NS; ++s) qf[s][0] = *reinterpret_cast<const u32x4 *>(qp + 16 * s);
+        } else {
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                float x[8];
+                if (a.q_dtype == FELLM_DTYPE_F32) load_f32<F32, 8>(static_cast<const float *>(a.q) + q0 + 16 * s, x);
+                else if (a.q_dtype == FELLM_DTYPE_F16) load_f32<F16, 8>(static_cast<const _Float16 *>(a.q) + q0 + 16 * s, x);
+                else load_f32<BF16, 8>(static_cast<const uint16_t *>(a.q) + q0 + 16 * s, x);
+#pragma unroll
+                for (int p = 0; p < QP; ++p)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) qf[s][p][w] = E::part(x[2 * w], x[2 * w + 1]);
+            }
+        }
+    }
+
+    f32x16 acc[ND];
+    float m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] = f32x16(0.0f);
+
+    // ---- staging: SK keys from kb + wave SK on
+    const uint32_t skey = lane / CH, spos = lane % CH;
+    auto stage = [&](uint32_t kb, uint8_t *kl, uint8_t *vl) {
+#pragma unroll
+        for (uint32_t b0 = 0; b0 < SK; b0 += (SK < kBlockTokens ? SK : kBlockTokens)) {
+            constexpr uint32_t BK = SK < kBlockTokens ? SK : kBlockTokens;
+            const uint32_t j = kb + wave * SK + b0;
+            const uint32_t have = j < sh.end ? min(BK, sh.end - j) : 0;
+            const uint8_t *kp = nullptr, *vp = nullptr;
+            if (have) {
+                kp = key_ptr<PAGED>(a, t, g, HD, j, false);
+                vp = key_ptr<PAGED>(a, t, g, HD, j, true);
+            }
+            const uint32_t ks = (PAGED ? a.stride : a.k_stride) * 2, vs = (PAGED ? a.stride : a.v_stride) * 2;
+            const Rsrc kr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(kp), 0,
+                                                              kp ? (int)((have - 1) * ks + RB) : 0, 0x00020000);
+            const Rsrc vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(vp), 0,
+                                                              vp ? (int)((have - 1) * vs + RB) : 0, 0x00020000);
+#pragma unroll
+            for (uint32_t i = 0; i < BK / KPI; ++i) {
+                const uint32_t key = i * KPI + skey;  // inside the piece of BK keys
+                const uint32_t c = (spos ^ swizzle<HD>(wave * SK + b0 + key)) * 16;
+                using L = __attribute__((address_space(3))) void;
+                const uint32_t at = (wave * SK + b0 + i * KPI) * RB;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (L *)(kl + at), 16, key * ks + c, 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (L *)(vl + at), 16, key * vs + c, 0, 0, 0);
+            }
+        }
+    };
+
+    // ---- one tile of KT keys from kb on
+    auto compute = [&](uint32_t kb, const uint8_t *kl, const uint8_t *vl) {
+        f32x16 s[NU];
+#pragma unroll
+        for (int u = 0; u < NU; ++u) s[u] = f32x16(0.0f);
+        const uint32_t kbase = kw * KT * RB + n * RB, ksw = (h ^ swizzle<HD>(n)) * 16;
+#pragma unroll
+        for (int st = 0; st < NS; ++st)
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                const u32x4 kf = *reinterpret_cast<const u32x4 *>(kl + kbase + u * 32 * RB + (ksw ^ (st * 32)));
+#pragma unroll
+                for (int p = 0; p < QP; ++p) s[u] = E::mfma(kf, qf[st][p], s[u]);
+            }
+        if (!(kb >= full_lo && kb + KT <= full_hi && kb + KT <= sh.end)) {
+            uint64_t bits = key_bits(a, t, token, mine, kb);
+            if (kb + 64 > sh.end) bits &= (1ull << (sh.end - kb)) - 1;
+            bits >>= 4 * h;
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!(bits >> (32 * u + 8 * (i / 4) + i % 4) & 1)) s[u][i] = -__builtin_inff();
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
+        top = halves_max(top);
+        if (__any((top - m) * a.c > kLazy)) {
+            const float mn = fmaxf(m, top);
+            const float f = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * a.c);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+        }
+        const float base = (m == -__builtin_inff() ? 0.0f : -m * a.c) + kBias;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], a.c, base));
+        float sum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum += s[u][i];
+        l += sum;
+        // V^T pieces: lane group of 16 reads keys 4 h + .. of dims 16 (group % 2) ..
+        const uint32_t vkey = 4 * h + lane % 16 / 4, vpc = lane / 16 % 2 * 2 + lane % 4 / 2;
+        const uint32_t vbase = kw * KT * RB + vkey * RB + lane % 2 * 8;
+        const uint32_t vsw0 = (vpc ^ swizzle<HD>(vkey)) * 16, vsw1 = (vpc ^ swizzle<HD>(vkey + 8)) * 16;
+        using L4 = __attribute__((address_space(3))) s16x4;
+#pragma unroll
+        for (int k = 0; k < KT / 16; ++k) {
+            u32x4 pf[PP];
+            {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = s[k / 2][8 * (k % 2) + e];
+#pragma unroll
+                for (int p = 0; p < PP; ++p)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) pf[p][w] = E::part(x[2 * w], x[2 * w + 1]);
+            }
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const uint32_t off = k * 16 * RB + vbase;
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L4 *)(vl + off + (vsw0 ^ (d * 64))));
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L4 *)(vl + off + 8 * RB + (vsw1 ^ (d * 64))));
+                const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
+                const u32x4 vf = {lo2[0], lo2[1], hi2[0], hi2[1]};
+#pragma unroll
+                for (int p = 0; p < PP; ++p) acc[d] = E::mfma(vf, pf[p], acc[d]);
+            }
+        }
+    };
+
+    auto round = [&](uint32_t kb, const uint8_t *kl, const uint8_t *vl, uint8_t *kn, uint8_t *vn) {
+        __syncthreads();  // this round's tiles have arrived, the other buffers are no longer read
+        if (kb + TK < sh.end) stage(kb + TK, kn, vn);
+        const uint32_t my = kb + kw * KT;
+        if (my < min(sh.end, any_hi) && my + KT > any_lo) compute(my, kl, vl);
+    };
+    if (sh.begin < sh.end) stage(sh.begin, k_lds0, v_lds0);
+    for (uint32_t kb = sh.begin; kb < sh.end; kb += 2 * TK) {
+        round(kb, k_lds0, v_lds0, k_lds1, v_lds1);
+        if (kb + TK < sh.end) round(kb + TK, k_lds1, v_lds1, k_lds0, v_lds0);
+    }
+    l = halves_sum(l);
+
+    // ---- wavefronts that share rows: merge into the first (through LDS, one at a time)
+    if constexpr (KW > 1) {
+        // tile d of the sums goes to the d-th of the four buffers in turn
+        static_assert(RW * kWave * 16 * 4 * ((ND + 3) / 4) <= TK * RB, "merge buffers");
+        __shared__ float ml_lds[RW * kWave * 2];
+        float *ml = ml_lds + rw * kWave * 2;
+        auto sum_at = [&](int d, int i) -> float & {
+            uint8_t *buf = d % 4 == 0 ? k_lds0 : d % 4 == 1 ? v_lds0 : d % 4 == 2 ? k_lds1 : v_lds1;
+            return reinterpret_cast<float *>(buf)[((d / 4 * RW + rw) * 16 + i) * kWave + lane];
+        };
+        for (int w = 1; w < KW; ++w) {
+            __syncthreads();
+            if (kw == (uint32_t)w) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum_at(d, i) = acc[d][i];
+                ml[lane] = m;
+                ml[kWave + lane] = l;
+            }
+            __syncthreads();
+            if (kw == 0) {
+                const float m2 = ml[lane], l2 = ml[kWave + lane];
+                const float mn = fmaxf(m, m2);
+                const float f1 = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * a.c);
+                const float f2 = m2 == mn ? 1.0f : __builtin_amdgcn_exp2f((m2 - mn) * a.c);
+                m = mn;
+                l = l * f1 + l2 * f2;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[d][i] = acc[d][i] * f1 + sum_at(d, i) * f2;
+            }
+        }
+        if (kw) return;
+    }
+
+    // ---- results
+    const bool direct = sh.live <= 1;
+    auto record = [&](uint32_t r) {  // of packed row r of the tile
+        return a.part + (((size_t)ti * a.n_kv + g) * a.splits + z) * BM * kRec<HD> + (size_t)r * kRec<HD>;
+    };
+    float probe = 0.0f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) probe = fmaf(acc[d][i], 0.0f, probe);
+    probe = halves_sum(probe) + l * 0.0f;
+    const bool bad = valid && !(probe == 0.0f && l > 0.0f);
+    if (valid && !bad) {
+        const float inv = direct ? 1.0f / l : 1.0f;
+        const size_t o0 = (size_t)(t.first + token) * a.out_stride + (size_t)head * HD + 4 * h;
+        float *rec = record(rw * kRows + n);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = acc[d][4 * i + e] * inv;
+                const uint32_t at = 32 * d + 8 * i;
+                if (!direct) store_f32<F32, 4>(rec + 4 * h + at, v);
+                else if (!PARTS || a.out_dtype != FELLM_DTYPE_F32) {
+                    if constexpr (!PARTS) {
+                        store_f32<typename E::A, 4>(static_cast<T *>(a.out) + o0 + at, v);
+                    } else if (a.out_dtype == FELLM_DTYPE_F16) {
+                        store_f32<F16, 4>(static_cast<_Float16 *>(a.out) + o0 + at, v);
+                    } else {
+                        store_f32<BF16, 4>(static_cast<uint16_t *>(a.out) + o0 + at, v);
+                    }
+                } else {
+                    store_f32<F32, 4>(static_cast<float *>(a.out) + o0 + at, v);
+                }
+            }
+        if (!direct && h == 0) {
+            rec[HD] = m;
+            rec[HD + 1] = l;
+        }
+    }
+    uint64_t again = __ballot(bad) & 0xffffffffull;
+    while (again) {
+        const uint32_t r = (uint32_t)__builtin_ctzll(again);
+        again &= again - 1;
+        const uint32_t pr = t.row0 + rw * kRows + r, tk = pr / a.group, hd = g * a.group + pr % a.group;
+        float sums[HD / 64], m1, l1;
+        careful_row<E, HD, PAGED>(a, t, g, tk, hd, sh.begin, sh.end, kBias, sums, m1, l1);
+        const bool none = m1 == -__builtin_inff() && l1 == 0.0f;  // no attended key
+        float *rec = record(rw * kRows + r);
+#pragma unroll
+        for (int e = 0; e < HD / 64; ++e) {
+            if (direct)
+                store_elem(a.out, a.out_dtype, (size_t)(t.first + tk) * a.out_stride + (size_t)hd * HD + lane + 64 * e,
+                           none ? 0.0f : sums[e] / l1);
+            else rec[lane + 64 * e] = sums[e];
+        }
+        if (!direct && lane == 0) {
+            rec[HD] = m1;
+            rec[HD + 1] = l1;
+        }
+    }
+}
+
+// Joins the splits' records of each row, one wavefront a row.
+template <int HD, uint32_t BM>
+__global__ __launch_bounds__(4 * kWave) void rows_combine(Args a) {
+    const uint32_t lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    constexpr uint32_t WG = BM / 4;  // workgroups per tile
+    const uint32_t r = blockIdx.x % WG * 4 + wave, id = blockIdx.x / WG;
+    const uint32_t g = id % a.n_kv, ti = id / a.n_kv;
+    const Tile t = find_tile<BM>(a, ti);
+    if (t.n == 0 || t.row0 + r >= t.n * a.group) return;
+    const Share sh = key_share<BM>(a, t, 0);
+    if (sh.live <= 1) return;
+    const float *rec = a.part + ((size_t)ti * a.n_kv + g) * a.splits * BM * kRec<HD> + (size_t)r * kRec<HD>;
+    const size_t step = (size_t)BM * kRec<HD>;
+    float top = -__builtin_inff();
+    for (uint32_t z = lane; z < sh.live; z += kWave) top = fmaxf(top, rec[z * step + HD]);
+    top = wave_max(top);
+    constexpr int PD = HD / 64;
+    float acc[PD] = {}, l = 0.0f;
+#pragma unroll 4
+    for (uint32_t z = 0; z < sh.live; ++z) {
+        const float *rz = rec + z * step;
+        const float mz = rz[HD], lz = rz[HD + 1];
+        const float f = mz == top ? 1.0f : __builtin_amdgcn_exp2f((mz - top) * a.c);
+        l = fmaf(lz, f, l);
+#pragma unroll
+        for (int e = 0; e < PD; ++e) acc[e] = fmaf(rz[lane + 64 * e], f, acc[e]);
+    }
+    const uint32_t pr = t.row0 + r, tk = pr / a.group, hd = g * a.group + pr % a.group;
+    const bool none = top == -__builtin_inff() && l == 0.0f;  // no attended key
+#pragma unroll
+    for (int e = 0; e < PD; ++e)
+        store_elem(a.out, a.out_dtype, (size_t)(t.first + tk) * a.out_stride + (size_t)hd * HD + lane + 64 * e,
+                   none ? 0.0f : acc[e] / l);
+}
+
+}  // namespace rows_attn
+}  // namespace fellm

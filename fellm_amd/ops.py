@@ -41,6 +41,40 @@ def _dev(*ts: torch.Tensor | None) -> None:
             raise ValueError("fellm_amd ops need contiguous tensors")
 
 
+def _rows(t: torch.Tensor, width: int | None = None) -> int:
+    """Row stride of a device matrix ``[rows, width]`` with dense rows, such as
+    a column slice of a projection's output."""
+    if not t.is_cuda:
+        raise ValueError("fellm_amd ops need device tensors (no CPU fallback)")
+    if t.dim() != 2 or (width is not None and t.shape[1] != width):
+        raise ValueError(f"expected a [rows, {width or 'width'}] tensor, got {tuple(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError("rows must be dense")
+    if t.shape[0] <= 1:
+        return t.shape[1]
+    if t.stride(0) < t.shape[1]:
+        raise ValueError("rows must not overlap")
+    return t.stride(0)
+
+
+def _u32(name: str, t: torch.Tensor | None, numel: int | None = None) -> None:
+    """An int32 tensor (read as u32) of numel elements."""
+    if t is None:
+        return
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32")
+    if numel is not None and t.numel() != numel:
+        raise ValueError(f"{name} must have {numel} elements, not {t.numel()}")
+
+
+def _same_device(first: torch.Tensor, *ts: torch.Tensor | None) -> None:
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise ValueError("tensors are on different devices")
+    if first.device.index != torch.cuda.current_device():
+        raise ValueError("tensors are not on the current device")
+
+
 def _p(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -228,6 +262,88 @@ def rope_kv_write(q, k, v, inv_freqs, kv_positions, cache: PagedKvCache, *, head
     return q_out
 
 
+def _norm_args(q, k, q_weight, k_weight, inv_freqs, head_dim, rope_dim):
+    """Checks shared by the per-head norm ops: (q stride, k stride, q heads, KV heads)."""
+    if head_dim <= 0 or q.shape[-1] % head_dim or k.shape[-1] % head_dim:
+        raise ValueError("q and k rows must be whole heads of head_dim")
+    qs, ks = _rows(q), _rows(k)
+    if q.shape[0] != k.shape[0] or q.dtype != k.dtype:
+        raise ValueError("q and k must have the same rows and dtype")
+    _dev(q_weight, k_weight, inv_freqs)
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w.dtype != torch.float32:
+            raise TypeError(f"{name} must be float32")
+        if w.numel() != head_dim:
+            raise ValueError(f"{name} must have head_dim elements")
+    if rope_dim:
+        if inv_freqs.dtype != torch.float32:
+            raise TypeError("inv_freqs must be float32")
+        if inv_freqs.numel() < rope_dim // 2:
+            raise ValueError("inv_freqs must have rope_dim / 2 elements")
+    return qs, ks, q.shape[1] // head_dim, k.shape[1] // head_dim
+
+
+def _rows_out(out, like):
+    """The output given for rows like `like`, checked, or a new dense one."""
+    if out is None:
+        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    if out.shape != like.shape or out.dtype != like.dtype:
+        raise ValueError("an output must have its input's shape and dtype")
+    return out
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, eps: float, inv_freqs, *, head_dim: int, rope_dim: int | None = None,
+                 pairing: int = 0, positions=None, position0: int = 0, q_out=None, k_out=None, inplace: bool = False):
+    """RMSNorm of every head of ``q`` and ``k``, then RoPE, in one pass.
+
+    ``q`` ``[rows, heads*head_dim]`` and ``k`` ``[rows, kv_heads*head_dim]`` may
+    be column slices of one projection.  ``q_weight`` and ``k_weight`` are f32
+    ``[head_dim]``; the rotation takes `rope`'s arguments.  Returns (q_out, k_out).
+    """
+    rope_dim = head_dim if rope_dim is None else rope_dim
+    qs, ks, nq, nk = _norm_args(q, k, q_weight, k_weight, inv_freqs, head_dim, rope_dim)
+    _dev(positions)
+    _u32("positions", positions, q.shape[0])
+    q_out = q if inplace else _rows_out(q_out, q)
+    k_out = k if inplace else _rows_out(k_out, k)
+    _same_device(q, k, q_weight, k_weight, inv_freqs, positions, q_out, k_out)
+    _lib.call("fellm_rocm_qk_norm_rope", _p(q), qs, _p(q_out), _rows(q_out), nq, _p(k), ks, _p(k_out), _rows(k_out), nk,
+              _code(q), q.shape[0], head_dim, rope_dim, pairing, _p(q_weight), _p(k_weight), eps, _p(inv_freqs),
+              _p(positions), position0, _stream())
+    return q_out, k_out
+
+
+def qk_norm_rope_kv_write(q, k, v, q_weight, k_weight, eps: float, inv_freqs, kv_positions, cache: PagedKvCache, *,
+                          head_dim: int, rope_dim: int | None = None, pairing: int = 0, rope_positions=None,
+                          sequences=None, layer: int = 0, q_out=None, k_out=None, inplace_q: bool = False,
+                          err_flag=None):
+    """`qk_norm_rope` fused with the paged append of the rotated K and of V.
+
+    Row r goes to ``kv_positions[r]`` of block-table row ``sequences[r]``
+    (default: r).  ``k_out``, if given, gets the rotated K rows.  Returns q_out.
+    """
+    rope_dim = head_dim if rope_dim is None else rope_dim
+    qs, ks, nq, nk = _norm_args(q, k, q_weight, k_weight, inv_freqs, head_dim, rope_dim)
+    rows = q.shape[0]
+    vs = _rows(v, k.shape[1])
+    if v.shape[0] != rows or v.dtype != q.dtype:
+        raise ValueError("v must have k's rows and dtype")
+    _dev(kv_positions, rope_positions, sequences, k_out, err_flag)
+    for name, t in (("kv_positions", kv_positions), ("rope_positions", rope_positions), ("sequences", sequences)):
+        _u32(name, t, rows)
+    _u32("err_flag", err_flag)
+    q_out = q if inplace_q else _rows_out(q_out, q)
+    if k_out is not None:
+        _rows_out(k_out, k)
+    _same_device(q, k, v, q_weight, k_weight, inv_freqs, kv_positions, rope_positions, sequences, q_out, k_out,
+                 cache.arena, cache.block_table, err_flag)
+    kv = cache.c_struct(layer)
+    _lib.call("fellm_rocm_qk_norm_rope_kv_write", _p(q), qs, _p(q_out), _rows(q_out), nq, _p(k), ks, _p(k_out), _p(v), vs,
+              nk, _code(q), rows, head_dim, rope_dim, pairing, _p(q_weight), _p(k_weight), eps, _p(inv_freqs),
+              _p(rope_positions), _p(kv_positions), _p(sequences), C.byref(kv), _p(err_flag), _stream())
+    return q_out
+
+
 def decode_step(q, k, v, inv_freqs, kv_positions, cache: PagedKvCache, x, residual, norm_weight, eps: float,
                 gate, up, *, head_dim: int, rope_dim: int | None = None, pairing: int = 0, rope_positions=None,
                 layer: int = 0, q_out=None, k_out=None, h_out=None, y_out=None, act_out=None, err_flag=None):
@@ -271,6 +387,76 @@ def paged_attention(q, row_lengths, cache: PagedKvCache, *, n_heads: int, n_kv_h
     _lib.call("fellm_rocm_paged_attention", _p(q), _code(q), _p(out), _code(out), batch, n_heads, n_kv_heads,
               head_dim, _p(row_lengths), max_seq, scale, int(causal), window, C.byref(kv), _p(workspace), ws_bytes,
               _stream())
+    return out
+
+
+def prompt_attention(q, k, v, cu_seqlens, *, n_heads: int, n_kv_heads: int, head_dim: int, scale: float = 0.0,
+                     causal: bool = True, window: int = 0, out=None):
+    """Attention of packed whole prompts: ``q`` ``[tokens, n_heads*head_dim]``,
+    ``k`` and ``v`` ``[tokens, n_kv_heads*head_dim]`` (f16 or bf16, row strides
+    allowed), ``cu_seqlens`` int32 device ``[sequences + 1]`` with the first
+    token of each sequence.  Returns out ``[tokens, n_heads*head_dim]``, in which
+    rows of no sequence are left as they were."""
+    qs = _rows(q, n_heads * head_dim)
+    ks, vs = (_rows(t, n_kv_heads * head_dim) for t in (k, v))
+    tokens = q.shape[0]
+    if any(t.shape[0] != tokens or t.dtype != q.dtype for t in (k, v)):
+        raise ValueError("q, k and v must have the same rows and dtype")
+    _dev(cu_seqlens, out)
+    _u32("cu_seqlens", cu_seqlens)
+    if cu_seqlens.numel() < 1:
+        raise ValueError("cu_seqlens must have sequences + 1 elements")
+    out = out if out is not None else torch.empty((tokens, n_heads * head_dim), dtype=q.dtype, device=q.device)
+    if out.numel() != tokens * n_heads * head_dim or out.dtype != q.dtype:
+        raise ValueError("out must have q's shape and dtype")
+    _same_device(q, k, v, cu_seqlens, out)
+    _lib.call("fellm_rocm_prompt_attention", _p(q), qs, _p(k), ks, _p(v), vs, _p(out), _code(q), _p(cu_seqlens),
+              cu_seqlens.numel() - 1, tokens, n_heads, n_kv_heads, head_dim, scale, int(causal), window, _stream())
+    return out
+
+
+def paged_tree_attention(q, cu_nodes, prefix_lengths, cache: PagedKvCache, *, n_heads: int, n_kv_heads: int,
+                         head_dim: int, max_nodes: int, max_prefix: int, tree_mask=None, layer: int = 0,
+                         scale: float = 0.0, window: int = 0, out=None, out_dtype=None, workspace=None):
+    """Attention of several new tokens a sequence over the paged cache, in which
+    their K and V stand after the prefix already.
+
+    ``q`` ``[tokens, n_heads*head_dim]``; sequence b's new tokens are the rows
+    ``cu_nodes[b] .. cu_nodes[b+1]`` behind ``prefix_lengths[b]`` cached ones
+    (int32 device ``[sequences + 1]`` and ``[sequences]``).  ``tree_mask`` int32
+    ``[tokens, words]``: bit j of a row's words says whether it attends its
+    sequence's new token j; None: causal (a chunk of a prompt), with an optional
+    ``window``.  ``max_nodes`` and ``max_prefix`` bound the counts.  Returns out
+    in out_dtype (default: q's dtype)."""
+    _dev(q, cu_nodes, prefix_lengths, tree_mask, out, workspace)
+    tokens = q.shape[0]
+    if q.numel() != tokens * n_heads * head_dim:
+        raise ValueError("q rows must be n_heads heads of head_dim")
+    _u32("cu_nodes", cu_nodes)
+    n_seqs = cu_nodes.numel() - 1
+    if n_seqs < 0:
+        raise ValueError("cu_nodes must have sequences + 1 elements")
+    _u32("prefix_lengths", prefix_lengths, n_seqs)
+    words = 0
+    if tree_mask is not None:
+        _u32("tree_mask", tree_mask)
+        if tree_mask.dim() != 2 or tree_mask.shape[0] != tokens:
+            raise ValueError("tree_mask must be [tokens, words]")
+        words = tree_mask.shape[1]
+    out_dtype = out_dtype or (q.dtype if out is None else out.dtype)
+    out = out if out is not None else torch.empty((tokens, n_heads * head_dim), dtype=out_dtype, device=q.device)
+    if out.numel() != q.numel() or out.dtype != out_dtype:
+        raise ValueError("out must have q's shape and the output dtype")
+    need = _lib.lib().fellm_rocm_paged_tree_attention_workspace(n_seqs, tokens, n_heads, n_kv_heads, head_dim, max_nodes,
+                                                                max_prefix)
+    if workspace is None and need:
+        workspace = torch.empty(need // 4, dtype=torch.float32, device=q.device)
+    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    _same_device(q, cu_nodes, prefix_lengths, tree_mask, out, workspace, cache.arena, cache.block_table)
+    kv = cache.c_struct(layer)
+    _lib.call("fellm_rocm_paged_tree_attention", _p(q), _code(q), _p(out), _code(out), _p(cu_nodes), _p(prefix_lengths),
+              n_seqs, tokens, _p(tree_mask), words, n_heads, n_kv_heads, head_dim, max_nodes, max_prefix, scale, window,
+              C.byref(kv), _p(workspace), ws_bytes, _stream())
     return out
 
 

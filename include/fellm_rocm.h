@@ -143,6 +143,48 @@ int fellm_rocm_rope_kv_write(const void *q, void *q_out, uint32_t n_q_heads, con
                              const FellmRocmPagedKv *kv, uint32_t *err_flag, void *stream);
 
 /*
+ * RMSNorm of every query and key head with RoPE in the same pass, for models
+ * that norm q and k per head (the reference runs RmsNorm over rows of head_dim
+ * and then Rope: backend.rs:1115-1124, :1135-1172).
+ * q: rows of n_q_heads heads of head_dim, q_stride elements apart; q_out the
+ * same with q_out_stride; k, k_out alike with n_kv_heads heads.  Strides let q,
+ * k and v be column slices of one projection.  An output may be its input
+ * (with the same stride) and must not overlap any input otherwise.
+ * Per head x: n = x / sqrt(mean(x^2) + eps) * weight (q_weight, k_weight: f32
+ * [head_dim]), then n is rotated as fellm_rocm_rope rotates x (rope_dim,
+ * pairing, positions / position0).  All f32, rounded once.  The angle is
+ * position * inv_freqs[i] exactly (f64 reduction), not rounded to f32 first as
+ * in fellm_rocm_rope: at far positions the two differ by that rounding.
+ * Any even head_dim; rope_dim even, <= min(head_dim, 1024).  Fast where
+ * head_dim and rope_dim are multiples of 16 (f32: 8), head_dim <= 512 (f32:
+ * 256), and pointers and rows 16-byte aligned.
+ */
+int fellm_rocm_qk_norm_rope(const void *q, uint32_t q_stride, void *q_out, uint32_t q_out_stride, uint32_t n_q_heads,
+                            const void *k, uint32_t k_stride, void *k_out, uint32_t k_out_stride,
+                            uint32_t n_kv_heads, uint32_t act_dtype, uint32_t rows, uint32_t head_dim,
+                            uint32_t rope_dim, uint32_t pairing, const float *q_weight, const float *k_weight,
+                            float eps, const float *inv_freqs, const uint32_t *positions, uint32_t position0,
+                            void *stream);
+
+/*
+ * The same with the paged K/V append of fellm_rocm_rope_kv_write: normed and
+ * rotated k and raw v are rounded once to kv->kv_dtype and stored at
+ * kv_positions[r] of block-table row sequences[r] (NULL: r), so a prompt's or a
+ * drafted tree's tokens share their sequence's table row.  k_out (dense rows)
+ * may be NULL; rope_positions NULL: kv_positions.  Rows of one call must name
+ * different slots.  A slot outside the arena or table sets *err_flag (device,
+ * may be NULL) and is skipped.
+ */
+int fellm_rocm_qk_norm_rope_kv_write(const void *q, uint32_t q_stride, void *q_out, uint32_t q_out_stride,
+                                     uint32_t n_q_heads, const void *k, uint32_t k_stride, void *k_out, const void *v,
+                                     uint32_t v_stride, uint32_t n_kv_heads, uint32_t act_dtype, uint32_t rows,
+                                     uint32_t head_dim, uint32_t rope_dim, uint32_t pairing, const float *q_weight,
+                                     const float *k_weight, float eps, const float *inv_freqs,
+                                     const uint32_t *rope_positions, const uint32_t *kv_positions,
+                                     const uint32_t *sequences, const FellmRocmPagedKv *kv, uint32_t *err_flag,
+                                     void *stream);
+
+/*
  * One decode step's memory-bound ops in a single launch: RoPE(q), RoPE(k) and
  * the paged K/V append (fellm_rocm_rope_kv_write's arguments), residual add +
  * RMSNorm with y in act_dtype (fellm_rocm_add_rmsnorm's), and SwiGLU
@@ -273,6 +315,66 @@ int fellm_rocm_paged_attention(const void *q, uint32_t q_dtype, void *out, uint3
                                uint32_t max_seq, float scale, uint32_t causal, uint32_t window,
                                const FellmRocmPagedKv *kv, float *workspace, uint64_t workspace_bytes,
                                void *stream);
+
+/*
+ * Attention of packed whole prompts: sequence b is the tokens cu_seqlens[b] ..
+ * cu_seqlens[b + 1] - 1 (u32 [n_seqs + 1], device, not decreasing) of q, k, v
+ * and out, `tokens` rows in all; rows of no sequence are left as they are.
+ * Token i of a sequence attends its tokens 0 .. i (causal; the last `window`
+ * of them when window > 0), or without causal all of them (those within
+ * `window` of it, |i - j| < window, when window > 0).  Query head h uses KV
+ * head h / (n_heads / n_kv_heads); out = softmax(q . k * scale) . v, scale <= 0
+ * meaning 1/sqrt(head_dim).
+ *   The reference's prefill runs its host attention per sequence
+ *   (backend.rs:1371-1397, attention_provider.rs:251-385).
+ * q [tokens, n_heads, head_dim] rows q_stride elements apart (k, v alike with
+ * n_kv_heads: column slices of a projection); out dense.  F16 or BF16, all the
+ * same; head_dim 64, 128 or 256; pointers 16-byte aligned, strides multiples of
+ * 8 and at most 2^26.  out must not overlap the inputs.
+ * Scores, softmax and sums are f32; a probability is rounded once to the input
+ * type for the product with v.  Only attended keys and values count, whatever
+ * masked ones hold: a row whose attended values are not finite gets what the
+ * formula gives.
+ */
+int fellm_rocm_prompt_attention(const void *q, uint32_t q_stride, const void *k, uint32_t k_stride, const void *v,
+                                uint32_t v_stride, void *out, uint32_t dtype, const uint32_t *cu_seqlens,
+                                uint32_t n_seqs, uint32_t tokens, uint32_t n_heads, uint32_t n_kv_heads,
+                                uint32_t head_dim, float scale, uint32_t causal, uint32_t window, void *stream);
+
+/*
+ * Attention of several new tokens per sequence over the paged cache: the
+ * verification of a drafted tree, or a chunk of a prompt behind its cached
+ * prefix.  Sequence b's new tokens are rows cu_nodes[b] .. cu_nodes[b + 1] - 1
+ * (u32 [n_seqs + 1], device) of q [tokens, n_heads, head_dim] and out; their K
+ * and V are in the cache already (fellm_rocm_qk_norm_rope_kv_write or
+ * fellm_rocm_kv_write), new token j at position prefix_lengths[b] + j of
+ * block-table row b.  Every new token attends the whole prefix (positions
+ * below prefix_lengths[b]), and of the new tokens those j whose bit is set in
+ * its row of tree_mask: bit j % 32 of word j / 32 (u32 [tokens, mask_words]; j
+ * past the words: not attended; a token attends itself only if its bit says
+ * so).  tree_mask NULL (mask_words 0): tokens j <= i, and with window > 0 only
+ * the last `window` positions.  A row without attended keys is zero.
+ * q F32, F16 or BF16, out the q dtype or F32, kv->kv_dtype F16 or BF16,
+ * head_dim 64, 128 or 256, kv->block_size 16.  max_nodes >= every sequence's
+ * new tokens and max_prefix >= every prefix length choose the launch; larger
+ * values than these on the device give right results, more slowly.
+ * workspace: fellm_rocm_paged_tree_attention_workspace() bytes, 16-byte
+ * aligned, for joining split keys; null or short: no split.  Calls that overlap
+ * need a workspace each.  Lengths past the table, and table entries outside the
+ * arena, read as zero keys and values.
+ * As paged decode attention, q and the probabilities are held in 16-bit parts
+ * to f32 accuracy when q or out is not of the cache's type; when all three are
+ * the same, each is used in that type, the probabilities rounded once.
+ */
+uint64_t fellm_rocm_paged_tree_attention_workspace(uint32_t n_seqs, uint32_t tokens, uint32_t n_heads,
+                                                   uint32_t n_kv_heads, uint32_t head_dim, uint32_t max_nodes,
+                                                   uint32_t max_prefix);
+int fellm_rocm_paged_tree_attention(const void *q, uint32_t q_dtype, void *out, uint32_t out_dtype,
+                                    const uint32_t *cu_nodes, const uint32_t *prefix_lengths, uint32_t n_seqs,
+                                    uint32_t tokens, const uint32_t *tree_mask, uint32_t mask_words, uint32_t n_heads,
+                                    uint32_t n_kv_heads, uint32_t head_dim, uint32_t max_nodes, uint32_t max_prefix,
+                                    float scale, uint32_t window, const FellmRocmPagedKv *kv, float *workspace,
+                                    uint64_t workspace_bytes, void *stream);
 
 /*
  * Attention over f32 K/V rows stored contiguously ([t, n_kv_heads * head_dim]):
