@@ -17,12 +17,37 @@ int launch_prompt(Args a, hipStream_t st) {
     return launch_status();
 }
 
+// Layouts (wavefronts that own rows, wavefronts that share them, keys of a
+// tile, wavefronts per SIMD) by the tiles of 128 rows that the launch could
+// have, w.  Few tiles: 64 rows a workgroup, two wavefronts on alternate keys,
+// which halves the longest walk.  Measured in us, the layouts compared in the
+// order of the lines below:
+//  64:  one prompt of 1024 tokens (32/8 heads, w 256) 15.4, 22.0; of 2048 (512)
+//       31.2, 40.3; of 4096 (1024) 91.9, 88.8; 16 of 256 (1024) 23.3, 17.4
+//  128: one prompt of 512 tokens (32/8 heads, w 128) 13.4, 16.9, 20.8, 20.9; of
+//       2048 (512) 55.4, 52.2, 65.4, 62.2; of 4096 (1024) 165, 151, 153, 142; 17
+//       of 128 .. 2048 (28/4, 2707) 194, 144, 134, 151; one of 16384 (32/4) 2357,
+//       2010, 2007, 1999
+//  256: one prompt of 1024 tokens (16/4 heads, w 128) 43, 63; of 2048 (256) 88,
+//       112; of 4096 (512) 290, 219; of 16384 (2048) 4073, 1941
+// Whole prompts of 16384 rows and more on average keep eight wavefronts busy on
+// the same keys; shorter ones gain more from a third workgroup on a CU, which
+// covers the others' starts and ends.
 template <typename E>
 int prompt_heads(uint32_t head_dim, const Args &a, hipStream_t st) {
-    if (head_dim == 64) return launch_prompt<E, 64, 4, 1, 64, 2>(a, st);
-    if (head_dim == 128) return launch_prompt<E, 128, 4, 1, 64, 2>(a, st);
-    if (head_dim == 256) return launch_prompt<E, 256, 4, 1, 32, 1>(a, st);
-    return FELLM_ERR_SHAPE;
+    const uint64_t rows = (uint64_t)a.tokens * a.group, w = (rows + 127) / 128 * a.n_kv;
+    if (head_dim == 64) {
+        if (w < 1024) return launch_prompt<E, 64, 2, 2, 32, 4>(a, st);
+        return launch_prompt<E, 64, 4, 1, 64, 2>(a, st);
+    }
+    if (head_dim == 128) {
+        if (w < 512) return launch_prompt<E, 128, 2, 2, 32, 2>(a, st);
+        if (w < 1024) return launch_prompt<E, 128, 4, 1, 64, 2>(a, st);
+        if (rows / a.n_seqs < 16384) return launch_prompt<E, 128, 4, 1, 32, 3>(a, st);
+        return launch_prompt<E, 128, 8, 1, 64, 2>(a, st);
+    }
+    if (w <= 256) return launch_prompt<E, 256, 2, 2, 32, 1>(a, st);
+    return launch_prompt<E, 256, 8, 1, 32, 2>(a, st);
 }
 
 }  // namespace

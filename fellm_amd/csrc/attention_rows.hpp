@@ -137,6 +137,71 @@ __device__ __forceinline__ Tile find_tile(const Args &a, uint32_t t) {
     return r;
 }
 
+// Sum of v over the wavefront, uniform.
+__device__ __forceinline__ uint32_t wave_total(uint32_t v) {
+    v += dpp_u32<0x140>(v);
+    v += dpp_u32<0x141>(v);
+    v += dpp_u32<0x4E>(v);
+    v += dpp_u32<0xB1>(v);
+    return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) +
+           __builtin_amdgcn_readlane(v, 48);
+}
+
+// The tile of the given rank when the tiles of all sequences are ordered by
+// their place in the sequence, the last first: under a causal mask those have
+// the most keys, and workgroups that start last should have the least to do.
+// (Seventeen f16 prompts of 128 to 2048 tokens, 28/4 heads of 128: 146 us with
+// the tiles in the order of the sequences.)  Up to 64 sequences, one a lane:
+// the level is found by search over sum_b max(0, T_b - level).
+template <uint32_t BM>
+__device__ __forceinline__ Tile ranked_tile(const Args &a, uint32_t rank) {
+    const uint32_t lane = threadIdx.x % kWave;
+    uint32_t first = 0, n = 0;
+    if (lane < a.n_seqs) {
+        first = min(a.cu[lane], a.tokens);
+        const uint32_t end = min(a.cu[lane + 1], a.tokens);
+        n = end > first ? end - first : 0;
+    }
+    const uint32_t tiles = (n * a.group + BM - 1) / BM;
+    Tile r{0, 0, 0, 0, 0};
+    uint32_t level, seq = 0;
+    if (a.n_seqs == 1) {
+        const uint32_t t0 = __builtin_amdgcn_readfirstlane(tiles);
+        if (rank >= t0) return r;
+        level = t0 - 1 - rank;
+    } else {
+        if (wave_total(tiles) <= rank) return r;
+        // tiles at levels >= lo: more than rank; >= hi: `above`, at most rank
+        uint32_t lo = 0, hi = a.tokens * a.group / BM + 1, above = 0;
+        while (hi - lo > 1) {
+            const uint32_t step = max(1u, (hi - lo) / 4);
+            uint32_t c[3];
+#pragma unroll
+            for (uint32_t i = 0; i < 3; ++i) {
+                const uint32_t at = lo + (i + 1) * step;
+                c[i] = wave_total(tiles > at ? tiles - at : 0);
+            }
+            const uint32_t base = lo, top = hi;
+#pragma unroll
+            for (uint32_t i = 0; i < 3; ++i) {
+                const uint32_t at = base + (i + 1) * step;
+                if (at >= top) continue;
+                if (c[i] > rank) lo = at;
+                else if (at < hi) hi = at, above = c[i];
+            }
+        }
+        level = lo;
+        uint64_t at = __ballot(tiles > level);
+        for (uint32_t k = rank - above; k; --k) at &= at - 1;
+        seq = (uint32_t)__builtin_ctzll(at);
+    }
+    r.seq = seq;
+    r.first = __builtin_amdgcn_readlane(first, seq);
+    r.n = __builtin_amdgcn_readlane(n, seq);
+    r.row0 = level * BM;
+    return r;
+}
+
 // Attended keys of token i: [lo, hi), all of them or, at and past `before`, those with a bit.
 struct KeyRange {
     uint32_t lo, hi;
@@ -281,6 +346,25 @@ __device__ __forceinline__ float halves_sum(float v) {
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
+// 32 dims of a row, lane h with dims 8 i + 4 h + e in v[4 i + e], as 16-bit
+// numbers: the row's two lanes exchange 4-dim pieces and store 8 dims each.
+template <typename O>
+__device__ __forceinline__ void store_tile(typename O::T *to, const f32x16 &v, uint32_t h) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        using H = typename HwStore<O>::type;
+        const typename O::T pair[2] = {H::store(v[2 * i]), H::store(v[2 * i + 1])};
+        memcpy(&w[i], pair, 4);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const auto a = __builtin_amdgcn_permlane32_swap(w[4 * j], w[4 * j + 2], false, false);
+        const auto b = __builtin_amdgcn_permlane32_swap(w[4 * j + 1], w[4 * j + 3], false, false);
+        *reinterpret_cast<u32x4 *>(to + 16 * j + 8 * h) = u32x4{a[0], b[0], a[1], b[1]};
+    }
+}
+
 // A split's partial record of one row: HD unnormalised sums, m, l, two unused.
 template <int HD>
 constexpr uint32_t kRec = HD + 4;
@@ -332,7 +416,7 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     const uint32_t z = blockIdx.x / per, id = blockIdx.x % per;
     const uint32_t g = id % a.n_kv, tiles = per / a.n_kv;
     const uint32_t ti = tiles - 1 - id / a.n_kv;
-    const Tile t = find_tile<BM>(a, ti);
+    const Tile t = !PAGED && a.n_seqs <= kWave ? ranked_tile<BM>(a, id / a.n_kv) : find_tile<BM>(a, ti);
     if (t.n == 0) return;
     const Share sh = key_share<BM>(a, t, z);
     if (z >= max(sh.live, 1u)) return;
@@ -347,6 +431,40 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     const KeyRange rf = row_keys(a, t, w0 / a.group), rl = row_keys(a, t, w1 / a.group);
     const uint32_t full_lo = rl.lo, full_hi = a.mask ? t.before : rf.hi, any_lo = rf.lo, any_hi = rl.hi;
 
+    f32x16 acc[ND];
+    float m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] = f32x16(0.0f);
+
+    // ---- staging: SK keys from kb + wave SK on
+    const uint32_t skey = lane / CH, spos = lane % CH;
+    auto stage = [&](uint32_t kb, uint8_t *lds, bool is_v) __attribute__((always_inline)) {
+        constexpr uint32_t BK = SK < kBlockTokens ? SK : kBlockTokens;
+#pragma unroll
+        for (uint32_t b0 = 0; b0 < SK; b0 += BK) {
+            const uint32_t j = kb + wave * SK + b0;
+            const uint32_t have = j < sh.end ? min(BK, sh.end - j) : 0;
+            const uint8_t *src = have ? key_ptr<PAGED>(a, t, g, HD, j, is_v) : nullptr;
+            const uint32_t stride = (PAGED ? a.stride : is_v ? a.v_stride : a.k_stride) * 2;
+            const Rsrc rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(src), 0,
+                                                              src ? (int)((have - 1) * stride + RB) : 0, 0x00020000);
+#pragma unroll
+            for (uint32_t i = 0; i < BK / KPI; ++i) {
+                const uint32_t key = i * KPI + skey;  // inside the piece of BK keys
+                const uint32_t c = (spos ^ swizzle<HD>(wave * SK + b0 + key)) * 16;
+                using L = __attribute__((address_space(3))) void;
+                const uint32_t at = (wave * SK + b0 + i * KPI) * RB;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (L *)(lds + at), 16, key * stride + c, 0, 0, 0);
+            }
+        }
+    };
+
+    if (sh.begin < sh.end) {
+        stage(sh.begin, k_lds0, false);
+        stage(sh.begin, v_lds0, true);
+    }
+
+    // Q^T as the B operand: row n, dims 16 st + 8 h .. +7
     u32x4 qf[NS][QP];
     {
         const size_t q0 = (size_t)(t.first + token) * a.q_stride + (size_t)head * HD + 8 * h;
@@ -369,47 +487,13 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
         }
     }
 
-    f32x16 acc[ND];
-    float m = -__builtin_inff(), l = 0.0f;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) acc[d] = f32x16(0.0f);
-
-    // ---- staging: SK keys from kb + wave SK on
-    const uint32_t skey = lane / CH, spos = lane % CH;
-    auto stage = [&](uint32_t kb, uint8_t *kl, uint8_t *vl) {
-#pragma unroll
-        for (uint32_t b0 = 0; b0 < SK; b0 += (SK < kBlockTokens ? SK : kBlockTokens)) {
-            constexpr uint32_t BK = SK < kBlockTokens ? SK : kBlockTokens;
-            const uint32_t j = kb + wave * SK + b0;
-            const uint32_t have = j < sh.end ? min(BK, sh.end - j) : 0;
-            const uint8_t *kp = nullptr, *vp = nullptr;
-            if (have) {
-                kp = key_ptr<PAGED>(a, t, g, HD, j, false);
-                vp = key_ptr<PAGED>(a, t, g, HD, j, true);
-            }
-            const uint32_t ks = (PAGED ? a.stride : a.k_stride) * 2, vs = (PAGED ? a.stride : a.v_stride) * 2;
-            const Rsrc kr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(kp), 0,
-                                                              kp ? (int)((have - 1) * ks + RB) : 0, 0x00020000);
-            const Rsrc vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(vp), 0,
-                                                              vp ? (int)((have - 1) * vs + RB) : 0, 0x00020000);
-#pragma unroll
-            for (uint32_t i = 0; i < BK / KPI; ++i) {
-                const uint32_t key = i * KPI + skey;  // inside the piece of BK keys
-                const uint32_t c = (spos ^ swizzle<HD>(wave * SK + b0 + key)) * 16;
-                using L = __attribute__((address_space(3))) void;
-                const uint32_t at = (wave * SK + b0 + i * KPI) * RB;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (L *)(kl + at), 16, key * ks + c, 0, 0, 0);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (L *)(vl + at), 16, key * vs + c, 0, 0, 0);
-            }
-        }
-    };
-
-    // ---- one tile of KT keys from kb on
-    auto compute = [&](uint32_t kb, const uint8_t *kl, const uint8_t *vl) {
-        f32x16 s[NU];
+    // ---- a tile of KT keys from kb on, in three parts
+    f32x16 s[NU];          // scores of row n
+    u32x4 pf[KT / 16][PP]; // probabilities, as the second product takes them
+    const uint32_t kbase = kw * KT * RB + n * RB, ksw = (h ^ swizzle<HD>(n)) * 16;
+    auto scores = [&](const uint8_t *kl) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) s[u] = f32x16(0.0f);
-        const uint32_t kbase = kw * KT * RB + n * RB, ksw = (h ^ swizzle<HD>(n)) * 16;
 #pragma unroll
         for (int st = 0; st < NS; ++st)
 #pragma unroll
@@ -418,6 +502,17 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
 #pragma unroll
                 for (int p = 0; p < QP; ++p) s[u] = E::mfma(kf, qf[st][p], s[u]);
             }
+        // K is read four pieces before its product: left alone, the compiler
+        // reads each right before it and waits for the LDS every time (one prompt
+        // of 16384 tokens, 32/4 heads of 128, bf16: 2114 -> 1939 us).
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int x = 0; x < NS * NU; ++x) {
+            __builtin_amdgcn_sched_group_barrier(0x008, QP, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+    };
+    auto weights = [&](uint32_t kb) __attribute__((always_inline)) {
         if (!(kb >= full_lo && kb + KT <= full_hi && kb + KT <= sh.end)) {
             uint64_t bits = key_bits(a, t, token, mine, kb);
             if (kb + 64 > sh.end) bits &= (1ull << (sh.end - kb)) - 1;
@@ -445,33 +540,30 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
                 for (int i = 0; i < 16; ++i) acc[d][i] *= f;
         }
         const float base = (m == -__builtin_inff() ? 0.0f : -m * a.c) + kBias;
-#pragma unroll
-        for (int u = 0; u < NU; ++u)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], a.c, base));
         float sum = 0.0f;
 #pragma unroll
-        for (int u = 0; u < NU; ++u)
+        for (int k = 0; k < KT / 16; ++k) {
+            float x[8];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sum += s[u][i];
+            for (int e = 0; e < 8; ++e) {
+                x[e] = __builtin_amdgcn_exp2f(fmaf(s[k / 2][8 * (k % 2) + e], a.c, base));
+                sum += x[e];
+            }
+#pragma unroll
+            for (int p = 0; p < PP; ++p)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) pf[k][p][w] = E::part(x[2 * w], x[2 * w + 1]);
+        }
         l += sum;
-        // V^T pieces: lane group of 16 reads keys 4 h + .. of dims 16 (group % 2) ..
-        const uint32_t vkey = 4 * h + lane % 16 / 4, vpc = lane / 16 % 2 * 2 + lane % 4 / 2;
-        const uint32_t vbase = kw * KT * RB + vkey * RB + lane % 2 * 8;
-        const uint32_t vsw0 = (vpc ^ swizzle<HD>(vkey)) * 16, vsw1 = (vpc ^ swizzle<HD>(vkey + 8)) * 16;
+    };
+    // V^T pieces: lane group of 16 reads keys 4 h + .. of dims 16 (group % 2) ..
+    const uint32_t vkey = 4 * h + lane % 16 / 4, vpc = lane / 16 % 2 * 2 + lane % 4 / 2;
+    const uint32_t vbase = kw * KT * RB + vkey * RB + lane % 2 * 8;
+    const uint32_t vsw0 = (vpc ^ swizzle<HD>(vkey)) * 16, vsw1 = (vpc ^ swizzle<HD>(vkey + 8)) * 16;
+    auto products = [&](const uint8_t *vl) __attribute__((always_inline)) {
         using L4 = __attribute__((address_space(3))) s16x4;
 #pragma unroll
-        for (int k = 0; k < KT / 16; ++k) {
-            u32x4 pf[PP];
-            {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = s[k / 2][8 * (k % 2) + e];
-#pragma unroll
-                for (int p = 0; p < PP; ++p)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) pf[p][w] = E::part(x[2 * w], x[2 * w + 1]);
-            }
+        for (int k = 0; k < KT / 16; ++k)
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
                 const uint32_t off = k * 16 * RB + vbase;
@@ -480,59 +572,87 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
                 const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
                 const u32x4 vf = {lo2[0], lo2[1], hi2[0], hi2[1]};
 #pragma unroll
-                for (int p = 0; p < PP; ++p) acc[d] = E::mfma(vf, pf[p], acc[d]);
+                for (int p = 0; p < PP; ++p) acc[d] = E::mfma(vf, pf[k][p], acc[d]);
             }
+    };
+    auto mine_at = [&](uint32_t kb) { return kb < min(sh.end, any_hi) && kb + KT > any_lo; };
+
+    // The wavefront's loads to LDS are done, then everyone's.  The wait is
+    // written out: a barrier alone does not imply it, and the one the compiler
+    // puts before the reads cannot know of other wavefronts' loads.
+    auto arrived = [&]() __attribute__((always_inline)) {
+        __asm__ volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), the other counters as they are
+        __asm__ volatile("" ::: "memory");
+        __syncthreads();
+    };
+    auto round = [&](uint32_t kb, const uint8_t *kl, const uint8_t *vl, uint8_t *kn, uint8_t *vn) __attribute__((always_inline)) {
+        arrived();  // this round's tiles are there, the other buffers are no longer read
+        if (kb + TK < sh.end) {
+            stage(kb + TK, kn, false);
+            stage(kb + TK, vn, true);
+        }
+        const uint32_t my = kb + kw * KT;
+        if (mine_at(my)) {
+            scores(kl);
+            weights(my);
+            products(vl);
         }
     };
-
-    auto round = [&](uint32_t kb, const uint8_t *kl, const uint8_t *vl, uint8_t *kn, uint8_t *vn) {
-        __syncthreads();  // this round's tiles have arrived, the other buffers are no longer read
-        if (kb + TK < sh.end) stage(kb + TK, kn, vn);
-        const uint32_t my = kb + kw * KT;
-        if (my < min(sh.end, any_hi) && my + KT > any_lo) compute(my, kl, vl);
-    };
-    if (sh.begin < sh.end) stage(sh.begin, k_lds0, v_lds0);
     for (uint32_t kb = sh.begin; kb < sh.end; kb += 2 * TK) {
         round(kb, k_lds0, v_lds0, k_lds1, v_lds1);
         if (kb + TK < sh.end) round(kb + TK, k_lds1, v_lds1, k_lds0, v_lds0);
     }
     l = halves_sum(l);
 
-    // ---- wavefronts that share rows: merge into the first (through LDS, one at a time)
+    float probe = 0.0f;  // NaN if any sum is not finite
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) probe = fmaf(acc[d][i], 0.0f, probe);
+    probe = halves_sum(probe) + l * 0.0f;
+
+    // ---- wavefronts that share rows: every one leaves its sums in LDS and
+    // joins (and stores) the tiles d = kw, kw + KW, .. of all of them
     if constexpr (KW > 1) {
-        // tile d of the sums goes to the d-th of the four buffers in turn
-        static_assert(RW * kWave * 16 * 4 * ((ND + 3) / 4) <= TK * RB, "merge buffers");
-        __shared__ float ml_lds[RW * kWave * 2];
-        float *ml = ml_lds + rw * kWave * 2;
-        auto sum_at = [&](int d, int i) -> float & {
-            uint8_t *buf = d % 4 == 0 ? k_lds0 : d % 4 == 1 ? v_lds0 : d % 4 == 2 ? k_lds1 : v_lds1;
-            return reinterpret_cast<float *>(buf)[((d / 4 * RW + rw) * 16 + i) * kWave + lane];
+        static_assert(16 * RW <= KT, "the sums of all wavefronts fit the four buffers");
+        __shared__ float state_lds[NW][3][kWave];
+        auto sum_at = [&](uint32_t w, int x) -> float & {  // x-th of a lane's 16 ND sums
+            uint8_t *buf = x < 4 * ND ? k_lds0 : x < 8 * ND ? v_lds0 : x < 12 * ND ? k_lds1 : v_lds1;
+            return reinterpret_cast<float *>(buf)[(w * 4 * ND + x % (4 * ND)) * kWave + lane];
         };
-        for (int w = 1; w < KW; ++w) {
-            __syncthreads();
-            if (kw == (uint32_t)w) {
+        __syncthreads();
 #pragma unroll
-                for (int d = 0; d < ND; ++d)
+        for (int d = 0; d < ND; ++d)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sum_at(d, i) = acc[d][i];
-                ml[lane] = m;
-                ml[kWave + lane] = l;
-            }
-            __syncthreads();
-            if (kw == 0) {
-                const float m2 = ml[lane], l2 = ml[kWave + lane];
-                const float mn = fmaxf(m, m2);
-                const float f1 = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * a.c);
-                const float f2 = m2 == mn ? 1.0f : __builtin_amdgcn_exp2f((m2 - mn) * a.c);
-                m = mn;
-                l = l * f1 + l2 * f2;
+            for (int i = 0; i < 16; ++i) sum_at(wave, d * 16 + i) = acc[d][i];
+        state_lds[wave][0][lane] = m;
+        state_lds[wave][1][lane] = l;
+        state_lds[wave][2][lane] = probe;
+        __syncthreads();
+        float f[KW];
+        m = -__builtin_inff();
 #pragma unroll
-                for (int d = 0; d < ND; ++d)
+        for (int w = 0; w < KW; ++w) m = fmaxf(m, state_lds[rw + w * RW][0][lane]);
+        l = probe = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[d][i] = acc[d][i] * f1 + sum_at(d, i) * f2;
+        for (int w = 0; w < KW; ++w) {
+            const float mw = state_lds[rw + w * RW][0][lane];
+            f[w] = mw == m ? 1.0f : __builtin_amdgcn_exp2f((mw - m) * a.c);
+            l = fmaf(state_lds[rw + w * RW][1][lane], f[w], l);
+            probe += state_lds[rw + w * RW][2][lane];
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            if (d % KW != (int)kw) continue;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float v = 0.0f;
+#pragma unroll
+                for (int w = 0; w < KW; ++w) v = fmaf(sum_at(rw + w * RW, d * 16 + i), f[w], v);
+                acc[d][i] = v;
             }
         }
-        if (kw) return;
     }
 
     // ---- results
@@ -540,43 +660,39 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     auto record = [&](uint32_t r) {  // of packed row r of the tile
         return a.part + (((size_t)ti * a.n_kv + g) * a.splits + z) * BM * kRec<HD> + (size_t)r * kRec<HD>;
     };
-    float probe = 0.0f;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) probe = fmaf(acc[d][i], 0.0f, probe);
-    probe = halves_sum(probe) + l * 0.0f;
     const bool bad = valid && !(probe == 0.0f && l > 0.0f);
+    // exchanges between a row's two lanes follow: both take part or neither, as
+    // valid and bad are the row's
     if (valid && !bad) {
         const float inv = direct ? 1.0f / l : 1.0f;
-        const size_t o0 = (size_t)(t.first + token) * a.out_stride + (size_t)head * HD + 4 * h;
+        const size_t o0 = (size_t)(t.first + token) * a.out_stride + (size_t)head * HD;
         float *rec = record(rw * kRows + n);
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
+        for (int d = 0; d < ND; ++d) {
+            if (KW > 1 && d % KW != (int)kw) continue;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float v[4];
+            for (int i = 0; i < 16; ++i) acc[d][i] *= inv;
+            if (!direct || (PARTS && a.out_dtype == FELLM_DTYPE_F32)) {
+                float *to = direct ? static_cast<float *>(a.out) + o0 : rec;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[d][4 * i + e] * inv;
-                const uint32_t at = 32 * d + 8 * i;
-                if (!direct) store_f32<F32, 4>(rec + 4 * h + at, v);
-                else if (!PARTS || a.out_dtype != FELLM_DTYPE_F32) {
-                    if constexpr (!PARTS) {
-                        store_f32<typename E::A, 4>(static_cast<T *>(a.out) + o0 + at, v);
-                    } else if (a.out_dtype == FELLM_DTYPE_F16) {
-                        store_f32<F16, 4>(static_cast<_Float16 *>(a.out) + o0 + at, v);
-                    } else {
-                        store_f32<BF16, 4>(static_cast<uint16_t *>(a.out) + o0 + at, v);
-                    }
-                } else {
-                    store_f32<F32, 4>(static_cast<float *>(a.out) + o0 + at, v);
+                for (int i = 0; i < 4; ++i) {
+                    const float v[4] = {acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+                    store_f32<F32, 4>(to + 32 * d + 8 * i + 4 * h, v);
                 }
+            } else if constexpr (!PARTS) {
+                store_tile<typename E::A>(static_cast<T *>(a.out) + o0 + 32 * d, acc[d], h);
+            } else if (a.out_dtype == FELLM_DTYPE_F16) {
+                store_tile<F16>(static_cast<_Float16 *>(a.out) + o0 + 32 * d, acc[d], h);
+            } else {
+                store_tile<BF16>(static_cast<uint16_t *>(a.out) + o0 + 32 * d, acc[d], h);
             }
-        if (!direct && h == 0) {
+        }
+        if (!direct && h == 0 && kw == 0) {
             rec[HD] = m;
             rec[HD + 1] = l;
         }
     }
+    if (kw) return;
     uint64_t again = __ballot(bad) & 0xffffffffull;
     while (again) {
         const uint32_t r = (uint32_t)__builtin_ctzll(again);

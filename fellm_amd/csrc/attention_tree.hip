@@ -19,9 +19,19 @@ struct Plan {
 };
 
 // Tiles of 32, 64 or 128 rows, the smallest that holds a sequence's rows: the
-// wavefronts without rows of their own share the keys.  The keys are split until the launch has
-// kTargetGroups workgroups, in parts of at least kMinKeys.
-constexpr uint32_t kTargetGroups = 512, kMinKeys = 256;
+// wavefronts without rows of their own share the keys.  The keys are split until
+// the launch has kTargetGroups workgroups, in parts of at least kMinKeys; the
+// keys of several sequences, whose lengths differ, in parts of at most kMaxKeys.
+#ifndef FELLM_TREE_GROUPS
+#define FELLM_TREE_GROUPS 512
+#endif
+#ifndef FELLM_TREE_MIN
+#define FELLM_TREE_MIN 128
+#endif
+#ifndef FELLM_TREE_MAX
+#define FELLM_TREE_MAX 2048
+#endif
+constexpr uint32_t kTargetGroups = FELLM_TREE_GROUPS, kMinKeys = FELLM_TREE_MIN, kMaxKeys = FELLM_TREE_MAX;
 
 Plan plan(uint32_t n_seqs, uint32_t tokens, uint32_t group, uint32_t n_kv, uint32_t max_nodes, uint32_t max_prefix) {
     Plan p;
@@ -33,7 +43,7 @@ Plan plan(uint32_t n_seqs, uint32_t tokens, uint32_t group, uint32_t n_kv, uint3
     const uint64_t used = std::min<uint64_t>(p.tiles, (uint64_t)n_seqs * ((rows + bm - 1) / bm)) * n_kv;
     const uint64_t keys = (uint64_t)max_prefix + max_nodes;
     uint64_t splits = std::min<uint64_t>((kTargetGroups + used - 1) / std::max<uint64_t>(used, 1), (keys + kMinKeys - 1) / kMinKeys);
-    splits = std::max<uint64_t>(splits, 1);
+    splits = std::max<uint64_t>(splits, n_seqs > 1 ? (keys + kMaxKeys - 1) / kMaxKeys : 1);
     if (splits == 1) {
         p.splits = 1;
         p.keys_per_split = 0x7fffffc0u;
@@ -53,12 +63,17 @@ uint64_t part_bytes(const Plan &p, uint32_t n_kv, uint32_t head_dim) {
 template <typename E, int HD, int RW, bool PARTS>
 int launch_tree(const Plan &p, const Args &a, hipStream_t st) {
     constexpr int KW = RW == 4 ? 1 : HD == 256 || RW == 2 ? 2 : 4;
-    constexpr int KT = RW == 4 && HD != 256 && !(PARTS && HD == 128) ? 64 : 32;
+    #ifndef TKT
+#define TKT 64
+#define TOCC 2
+#endif
+    constexpr int KT = RW == 4 && HD != 256 && !(PARTS && HD == 128) ? (HD == 128 ? TKT : 64) : 32;
+    constexpr int OCC = RW == 4 && HD <= 128 && !PARTS ? (HD == 128 ? TOCC : 2) : 1;
     constexpr uint32_t BM = kRows * RW;
     const uint64_t grid = p.tiles * a.n_kv * a.splits;
     // a launch has fewer than 2^32 threads
     if (std::max(grid, p.tiles * a.n_kv * (BM / 4)) > 0xffffffffull / (4 * kWave)) return FELLM_ERR_SHAPE;
-    FELLM_LAUNCH((rows_kernel<E, HD, RW, KW, KT, true, PARTS, 1>), dim3((uint32_t)grid), dim3(kWave * RW * KW), 0, st, a);
+    FELLM_LAUNCH((rows_kernel<E, HD, RW, KW, KT, true, PARTS, OCC>), dim3((uint32_t)grid), dim3(kWave * RW * KW), 0, st, a);
     int rc = launch_status();
     if (rc != FELLM_OK || a.splits == 1) return rc;
     FELLM_LAUNCH((rows_combine<HD, BM>), dim3((uint32_t)(p.tiles * a.n_kv * (BM / 4))), dim3(4 * kWave), 0, st, a);
