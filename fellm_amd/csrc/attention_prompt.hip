@@ -10,7 +10,7 @@ using namespace rows_attn;
 template <typename E, int HD, int RW, int KW, int KT, int OCC>
 int launch_prompt(Args a, hipStream_t st) {
     constexpr uint32_t BM = kRows * RW;
-    const uint64_t tiles = (uint64_t)a.tokens * a.group / BM + a.n_seqs;
+    const uint64_t rows = (uint64_t)a.tokens * a.group, tiles = a.n_seqs == 1 ? (rows + BM - 1) / BM : rows / BM + a.n_seqs;
     if (tiles * a.n_kv > 0xffffffffull / (kWave * RW * KW)) return FELLM_ERR_SHAPE;
     FELLM_LAUNCH((rows_kernel<E, HD, RW, KW, KT, false, false, OCC>), dim3((uint32_t)tiles * a.n_kv),
                  dim3(kWave * RW * KW), 0, st, a);

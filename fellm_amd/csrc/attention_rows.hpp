@@ -27,7 +27,8 @@
 //    rescaling of O.
 // A masked score is -inf before the exp; a masked V that is not finite makes
 // 0 x inf = NaN in the product, so rows whose result is not finite (or whose
-// sum is zero) are computed again key by key, over their attended keys alone.
+// sum is zero though they attend keys) are computed again key by key, over their
+// attended keys alone.  A row without keys is zero.
 #pragma once
 
 #include "common.hpp"
@@ -147,12 +148,21 @@ __device__ __forceinline__ uint32_t wave_total(uint32_t v) {
            __builtin_amdgcn_readlane(v, 48);
 }
 
+__device__ __forceinline__ uint32_t wave_most(uint32_t v) {
+    v = dpp_max_group<16>(v);
+    return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+               max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+
 // The tile of the given rank when the tiles of all sequences are ordered by
 // their place in the sequence, the last first: under a causal mask those have
 // the most keys, and workgroups that start last should have the least to do.
 // (Seventeen f16 prompts of 128 to 2048 tokens, 28/4 heads of 128: 146 us with
-// the tiles in the order of the sequences.)  Up to 64 sequences, one a lane:
-// the level is found by search over sum_b max(0, T_b - level).
+// the tiles in the order of the sequences.)  It also numbers the tiles without
+// gaps: workgroups are dealt to the shader engines in turn, and with every
+// second one empty half of the CUs had no work (16 drafted tokens behind 32768,
+// 32/8 heads of 128: 95 us).  Up to 64 sequences, one a lane: the level is
+// found by search over sum_b max(0, T_b - level).
 template <uint32_t BM>
 __device__ __forceinline__ Tile ranked_tile(const Args &a, uint32_t rank) {
     const uint32_t lane = threadIdx.x % kWave;
@@ -172,7 +182,7 @@ __device__ __forceinline__ Tile ranked_tile(const Args &a, uint32_t rank) {
     } else {
         if (wave_total(tiles) <= rank) return r;
         // tiles at levels >= lo: more than rank; >= hi: `above`, at most rank
-        uint32_t lo = 0, hi = a.tokens * a.group / BM + 1, above = 0;
+        uint32_t lo = 0, hi = wave_most(tiles), above = 0;
         while (hi - lo > 1) {
             const uint32_t step = max(1u, (hi - lo) / 4);
             uint32_t c[3];
@@ -199,7 +209,13 @@ __device__ __forceinline__ Tile ranked_tile(const Args &a, uint32_t rank) {
     r.first = __builtin_amdgcn_readlane(first, seq);
     r.n = __builtin_amdgcn_readlane(n, seq);
     r.row0 = level * BM;
+    r.before = a.before ? min(a.before[seq], a.max_before) : 0;
     return r;
+}
+
+template <uint32_t BM>
+__device__ __forceinline__ Tile tile_of(const Args &a, uint32_t rank, uint32_t tiles) {
+    return a.n_seqs <= kWave ? ranked_tile<BM>(a, rank) : find_tile<BM>(a, tiles - 1 - rank);
 }
 
 // Attended keys of token i: [lo, hi), all of them or, at and past `before`, those with a bit.
@@ -244,18 +260,23 @@ __device__ __forceinline__ uint64_t key_bits(const Args &a, const Tile &t, uint3
     return bits;
 }
 
+// Table entry of cache block `blk` of the sequence, ~0 where the table has none,
+// and the block's address, null where the arena has none.
+__device__ __forceinline__ uint32_t block_entry(const Args &a, const Tile &t, uint32_t blk) {
+    const size_t ti = ((size_t)t.seq * a.n_layers + a.layer) * a.n_logical + blk;
+    return blk < a.n_logical && ti < a.n_table ? a.table[ti] : ~0u;
+}
+__device__ __forceinline__ const uint8_t *block_ptr(const Args &a, uint32_t entry) {
+    return ((uint64_t)entry + 1) * a.block_bytes <= a.arena_len ? a.arena + entry * a.block_bytes : nullptr;
+}
+
 // Element pointers of key j (byte address), or null where the cache has no such block.
 template <bool PAGED>
 __device__ __forceinline__ const uint8_t *key_ptr(const Args &a, const Tile &t, uint32_t g, uint32_t hd, uint32_t j,
                                                   bool is_v) {
     if constexpr (PAGED) {
-        const uint32_t blk = j / kBlockTokens;
-        const size_t ti = ((size_t)t.seq * a.n_layers + a.layer) * a.n_logical + blk;
-        if (blk >= a.n_logical || ti >= a.n_table) return nullptr;
-        const uint64_t p = a.table[ti];
-        if ((p + 1) * a.block_bytes > a.arena_len) return nullptr;
-        return a.arena + p * a.block_bytes +
-               ((uint64_t)(j % kBlockTokens + (is_v ? kBlockTokens : 0)) * a.stride + (uint64_t)g * hd) * 2;
+        const uint8_t *at = block_ptr(a, block_entry(a, t, j / kBlockTokens));
+        return at ? at + ((uint64_t)(j % kBlockTokens + (is_v ? kBlockTokens : 0)) * a.stride + (uint64_t)g * hd) * 2 : nullptr;
     } else {
         const uint32_t stride = is_v ? a.v_stride : a.k_stride;
         return (is_v ? a.v : a.k) + ((size_t)(t.first + j) * stride + (size_t)g * hd) * 2;
@@ -389,11 +410,24 @@ __device__ __forceinline__ Share key_share(const Args &a, const Tile &t, uint32_
     return s;
 }
 
+// A buffer resource in scalar registers: everything it is made of is the same in
+// all lanes, but where the compiler does not see that it would loop over lanes
+// for every load (a chunk of 512 tokens behind 32256 keys: 340 us).
+__device__ __forceinline__ Rsrc uniform_rsrc(const uint8_t *p, uint32_t range) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint64_t u = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(v >> 32)) << 32 |
+                       (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)v);
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(u), 0, (int)__builtin_amdgcn_readfirstlane(range),
+                                             0x00020000);
+}
+
 // E: K/V policy, HD: head dim, RW: wavefronts that own 32 rows each, KW:
 // wavefronts that share those rows and take every KW-th key tile, KT: keys of
 // a wavefront's tile (32 or 64), PARTS: q and p held to f32 accuracy in several
 // 16-bit parts (q or out in f32, or q of another 16-bit type than K/V).
-template <typename E, int HD, int RW, int KW, int KT, bool PAGED, bool PARTS, int OCC>
+// OCC: wavefronts per SIMD the registers are kept for.  NST: key tiles in LDS
+// (NST - 1 on their way while one is worked on).
+template <typename E, int HD, int RW, int KW, int KT, bool PAGED, bool PARTS, int OCC, int NST = 2>
 __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     constexpr int NW = RW * KW, NS = HD / 16, NU = KT / 32, ND = HD / 32;
     constexpr int QP = PARTS ? E::kQParts : 1, PP = PARTS ? E::kPParts : 1;
@@ -405,7 +439,10 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     static_assert(SK % KPI == 0 && (SK <= kBlockTokens || SK % kBlockTokens == 0) && 64 % SK == 0);
     using T = typename E::A::T;
 
+    // Separate arrays: the compiler then knows that a read of one need not wait
+    // for loads to another.
     __shared__ __align__(16) uint8_t k_lds0[TK * RB], v_lds0[TK * RB], k_lds1[TK * RB], v_lds1[TK * RB];
+    __shared__ __align__(16) uint8_t k_lds2[NST > 2 ? TK * RB : 16], v_lds2[NST > 2 ? TK * RB : 16];
 
     const uint32_t lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const uint32_t rw = wave % RW, kw = wave / RW;
@@ -415,8 +452,8 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     const uint32_t per = gridDim.x / a.splits;
     const uint32_t z = blockIdx.x / per, id = blockIdx.x % per;
     const uint32_t g = id % a.n_kv, tiles = per / a.n_kv;
-    const uint32_t ti = tiles - 1 - id / a.n_kv;
-    const Tile t = !PAGED && a.n_seqs <= kWave ? ranked_tile<BM>(a, id / a.n_kv) : find_tile<BM>(a, ti);
+    const uint32_t ti = id / a.n_kv;
+    const Tile t = tile_of<BM>(a, ti, tiles);
     if (t.n == 0) return;
     const Share sh = key_share<BM>(a, t, z);
     if (z >= max(sh.live, 1u)) return;
@@ -433,21 +470,42 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
 
     f32x16 acc[ND];
     float m = -__builtin_inff(), l = 0.0f;
+    bool some = false;  // the row attends a key of this share
 #pragma unroll
     for (int d = 0; d < ND; ++d) acc[d] = f32x16(0.0f);
 
     // ---- staging: SK keys from kb + wave SK on
     const uint32_t skey = lane / CH, spos = lane % CH;
+    constexpr uint32_t BK = SK < kBlockTokens ? SK : kBlockTokens;  // keys of a piece, of one cache block
+    // Table entries of the pieces of the tile that is requested next (paged): read
+    // a tile ahead, so that their latency does not stand before the request.
+    uint32_t entry[SK / BK];
+    auto look_up = [&](uint32_t kb) __attribute__((always_inline)) {
+        if constexpr (PAGED) {
+#pragma unroll
+            for (uint32_t b = 0; b < SK / BK; ++b) {
+                // through a vector load: a scalar one on its way would turn every
+                // wait for an LDS read into a wait for all of them
+                uint32_t blk = (kb + wave * SK + b * BK) / kBlockTokens;
+                __asm__("" : "+v"(blk));
+                entry[b] = block_entry(a, t, blk);
+            }
+        }
+    };
     auto stage = [&](uint32_t kb, uint8_t *lds, bool is_v) __attribute__((always_inline)) {
-        constexpr uint32_t BK = SK < kBlockTokens ? SK : kBlockTokens;
 #pragma unroll
         for (uint32_t b0 = 0; b0 < SK; b0 += BK) {
             const uint32_t j = kb + wave * SK + b0;
             const uint32_t have = j < sh.end ? min(BK, sh.end - j) : 0;
-            const uint8_t *src = have ? key_ptr<PAGED>(a, t, g, HD, j, is_v) : nullptr;
             const uint32_t stride = (PAGED ? a.stride : is_v ? a.v_stride : a.k_stride) * 2;
-            const Rsrc rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(src), 0,
-                                                              src ? (int)((have - 1) * stride + RB) : 0, 0x00020000);
+            const uint8_t *src;
+            if constexpr (PAGED) {
+                const uint8_t *at = block_ptr(a, __builtin_amdgcn_readfirstlane(entry[b0 / BK]));
+                src = at ? at + (j % kBlockTokens + (is_v ? kBlockTokens : 0)) * stride + g * RB : nullptr;
+            } else {
+                src = key_ptr<PAGED>(a, t, g, HD, j, is_v);
+            }
+            const Rsrc rs = uniform_rsrc(src, src && have ? (have - 1) * stride + RB : 0);
 #pragma unroll
             for (uint32_t i = 0; i < BK / KPI; ++i) {
                 const uint32_t key = i * KPI + skey;  // inside the piece of BK keys
@@ -458,11 +516,16 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
             }
         }
     };
+    auto request = [&](uint32_t kb, uint8_t *kl, uint8_t *vl) __attribute__((always_inline)) {
+        if (kb >= sh.end) return;
+        stage(kb, kl, false);
+        stage(kb, vl, true);
+        look_up(kb + TK);
+    };
 
-    if (sh.begin < sh.end) {
-        stage(sh.begin, k_lds0, false);
-        stage(sh.begin, v_lds0, true);
-    }
+    look_up(sh.begin);
+    request(sh.begin, k_lds0, v_lds0);
+    if constexpr (NST > 2) request(sh.begin + TK, k_lds1, v_lds1);
 
     // Q^T as the B operand: row n, dims 16 st + 8 h .. +7
     u32x4 qf[NS][QP];
@@ -492,36 +555,41 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     u32x4 pf[KT / 16][PP]; // probabilities, as the second product takes them
     const uint32_t kbase = kw * KT * RB + n * RB, ksw = (h ^ swizzle<HD>(n)) * 16;
     auto scores = [&](const uint8_t *kl) __attribute__((always_inline)) {
+        // Piece x: dims 16 (x / NU) .. of keys 32 (x % NU) ...  Each is read kAhead
+        // products early and the order is fixed: left to itself the compiler reads
+        // a piece right before its product and waits for the LDS every time (one
+        // prompt of 16384 tokens, 32/4 heads of 128, bf16: 2114 -> 1939 us).
+        constexpr int N = NS * NU, kAhead = 4;
+        auto piece = [&](int x) {
+            return *reinterpret_cast<const u32x4 *>(kl + kbase + x % NU * 32 * RB + (ksw ^ (x / NU * 32)));
+        };
+        u32x4 kf[kAhead];
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) kf[x] = piece(x);
 #pragma unroll
         for (int u = 0; u < NU; ++u) s[u] = f32x16(0.0f);
 #pragma unroll
-        for (int st = 0; st < NS; ++st)
+        for (int x = 0; x < N; ++x) {
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int u = 0; u < NU; ++u) {
-                const u32x4 kf = *reinterpret_cast<const u32x4 *>(kl + kbase + u * 32 * RB + (ksw ^ (st * 32)));
-#pragma unroll
-                for (int p = 0; p < QP; ++p) s[u] = E::mfma(kf, qf[st][p], s[u]);
-            }
-        // K is read four pieces before its product: left alone, the compiler
-        // reads each right before it and waits for the LDS every time (one prompt
-        // of 16384 tokens, 32/4 heads of 128, bf16: 2114 -> 1939 us).
-        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-        for (int x = 0; x < NS * NU; ++x) {
-            __builtin_amdgcn_sched_group_barrier(0x008, QP, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            for (int p = 0; p < QP; ++p) s[x % NU] = E::mfma(kf[x % kAhead], qf[x / NU][p], s[x % NU]);
+            if (x + kAhead < N) kf[x % kAhead] = piece(x + kAhead);
         }
+        __builtin_amdgcn_sched_barrier(0);
     };
     auto weights = [&](uint32_t kb) __attribute__((always_inline)) {
         if (!(kb >= full_lo && kb + KT <= full_hi && kb + KT <= sh.end)) {
             uint64_t bits = key_bits(a, t, token, mine, kb);
             if (kb + 64 > sh.end) bits &= (1ull << (sh.end - kb)) - 1;
+            some |= (KT == 64 ? bits : (uint32_t)bits) != 0;
             bits >>= 4 * h;
 #pragma unroll
             for (int u = 0; u < NU; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (!(bits >> (32 * u + 8 * (i / 4) + i % 4) & 1)) s[u][i] = -__builtin_inff();
+        } else {
+            some = true;
         }
         float top = s[0][0];
 #pragma unroll
@@ -575,23 +643,28 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
                 for (int p = 0; p < PP; ++p) acc[d] = E::mfma(vf, pf[k][p], acc[d]);
             }
     };
-    auto mine_at = [&](uint32_t kb) { return kb < min(sh.end, any_hi) && kb + KT > any_lo; };
+    const uint32_t hi_here = t.row0 + rw * kRows < t.n * a.group ? min(sh.end, any_hi) : 0;  // 0: no row of its own
+    auto mine_at = [&](uint32_t kb) { return kb < hi_here && kb + KT > any_lo; };
 
-    // The wavefront's loads to LDS are done, then everyone's.  The wait is
+    // The oldest tile's loads to LDS are done, then everyone's.  The wait is
     // written out: a barrier alone does not imply it, and the one the compiler
-    // puts before the reads cannot know of other wavefronts' loads.
-    auto arrived = [&]() __attribute__((always_inline)) {
+    // puts before the reads cannot know of other wavefronts' loads.  Loads finish
+    // in order, so those of the NST - 2 tiles requested later may still be on
+    // their way (`newer`: there are such).
+    constexpr int kLater = (NST - 2) * 2 * (int)(SK / KPI);
+    static_assert(NST <= 3 && kLater < 16);
+    auto arrived = [&](bool newer) __attribute__((always_inline)) {
         __asm__ volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), the other counters as they are
+        if (NST > 2 && newer) __builtin_amdgcn_s_waitcnt(0x0f70 | kLater);  // vmcnt(kLater)
+        else __builtin_amdgcn_s_waitcnt(0x0f70);                            // vmcnt(0)
         __asm__ volatile("" ::: "memory");
         __syncthreads();
     };
+    // kn and vn: the buffers of the tile before, which no wavefront reads any more after the barrier
     auto round = [&](uint32_t kb, const uint8_t *kl, const uint8_t *vl, uint8_t *kn, uint8_t *vn) __attribute__((always_inline)) {
-        arrived();  // this round's tiles are there, the other buffers are no longer read
-        if (kb + TK < sh.end) {
-            stage(kb + TK, kn, false);
-            stage(kb + TK, vn, true);
-        }
+        if (kb >= sh.end) return;
+        arrived(kb + TK < sh.end);
+        request(kb + (NST - 1) * TK, kn, vn);
         const uint32_t my = kb + kw * KT;
         if (mine_at(my)) {
             scores(kl);
@@ -599,9 +672,15 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
             products(vl);
         }
     };
-    for (uint32_t kb = sh.begin; kb < sh.end; kb += 2 * TK) {
-        round(kb, k_lds0, v_lds0, k_lds1, v_lds1);
-        if (kb + TK < sh.end) round(kb + TK, k_lds1, v_lds1, k_lds0, v_lds0);
+    for (uint32_t kb = sh.begin; kb < sh.end; kb += NST * TK) {
+        if constexpr (NST == 2) {
+            round(kb, k_lds0, v_lds0, k_lds1, v_lds1);
+            round(kb + TK, k_lds1, v_lds1, k_lds0, v_lds0);
+        } else {
+            round(kb, k_lds0, v_lds0, k_lds2, v_lds2);
+            round(kb + TK, k_lds1, v_lds1, k_lds0, v_lds0);
+            round(kb + 2 * TK, k_lds2, v_lds2, k_lds1, v_lds1);
+        }
     }
     l = halves_sum(l);
 
@@ -616,7 +695,7 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     // joins (and stores) the tiles d = kw, kw + KW, .. of all of them
     if constexpr (KW > 1) {
         static_assert(16 * RW <= KT, "the sums of all wavefronts fit the four buffers");
-        __shared__ float state_lds[NW][3][kWave];
+        __shared__ float state_lds[NW][4][kWave];
         auto sum_at = [&](uint32_t w, int x) -> float & {  // x-th of a lane's 16 ND sums
             uint8_t *buf = x < 4 * ND ? k_lds0 : x < 8 * ND ? v_lds0 : x < 12 * ND ? k_lds1 : v_lds1;
             return reinterpret_cast<float *>(buf)[(w * 4 * ND + x % (4 * ND)) * kWave + lane];
@@ -629,6 +708,7 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
         state_lds[wave][0][lane] = m;
         state_lds[wave][1][lane] = l;
         state_lds[wave][2][lane] = probe;
+        state_lds[wave][3][lane] = some ? 1.0f : 0.0f;
         __syncthreads();
         float f[KW];
         m = -__builtin_inff();
@@ -641,6 +721,7 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
             f[w] = mw == m ? 1.0f : __builtin_amdgcn_exp2f((mw - m) * a.c);
             l = fmaf(state_lds[rw + w * RW][1][lane], f[w], l);
             probe += state_lds[rw + w * RW][2][lane];
+            some |= state_lds[rw + w * RW][3][lane] != 0.0f;
         }
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
@@ -660,11 +741,11 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     auto record = [&](uint32_t r) {  // of packed row r of the tile
         return a.part + (((size_t)ti * a.n_kv + g) * a.splits + z) * BM * kRec<HD> + (size_t)r * kRec<HD>;
     };
-    const bool bad = valid && !(probe == 0.0f && l > 0.0f);
+    const bool bad = valid && some && !(probe == 0.0f && l > 0.0f);
     // exchanges between a row's two lanes follow: both take part or neither, as
     // valid and bad are the row's
     if (valid && !bad) {
-        const float inv = direct ? 1.0f / l : 1.0f;
+        const float inv = !direct ? 1.0f : some ? 1.0f / l : 0.0f;
         const size_t o0 = (size_t)(t.first + token) * a.out_stride + (size_t)head * HD;
         float *rec = record(rw * kRows + n);
 #pragma unroll
@@ -716,24 +797,24 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     }
 }
 
-// Joins the splits' records of each row, one wavefront a row.
+// Joins the splits' records: 16 lanes a row, 16 rows a workgroup.
+constexpr uint32_t kJoinRows = 16;
 template <int HD, uint32_t BM>
-__global__ __launch_bounds__(4 * kWave) void rows_combine(Args a) {
-    const uint32_t lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    constexpr uint32_t WG = BM / 4;  // workgroups per tile
-    const uint32_t r = blockIdx.x % WG * 4 + wave, id = blockIdx.x / WG;
-    const uint32_t g = id % a.n_kv, ti = id / a.n_kv;
-    const Tile t = find_tile<BM>(a, ti);
+__global__ __launch_bounds__(kJoinRows * 16) void rows_combine(Args a) {
+    const uint32_t id = blockIdx.x / (BM / kJoinRows), g = id % a.n_kv, ti = id / a.n_kv;
+    const uint32_t r = blockIdx.x % (BM / kJoinRows) * kJoinRows + threadIdx.x / 16, col = threadIdx.x % 16;
+    const Tile t = tile_of<BM>(a, ti, gridDim.x / (BM / kJoinRows) / a.n_kv);
     if (t.n == 0 || t.row0 + r >= t.n * a.group) return;
     const Share sh = key_share<BM>(a, t, 0);
     if (sh.live <= 1) return;
     const float *rec = a.part + ((size_t)ti * a.n_kv + g) * a.splits * BM * kRec<HD> + (size_t)r * kRec<HD>;
     const size_t step = (size_t)BM * kRec<HD>;
     float top = -__builtin_inff();
-    for (uint32_t z = lane; z < sh.live; z += kWave) top = fmaxf(top, rec[z * step + HD]);
-    top = wave_max(top);
-    constexpr int PD = HD / 64;
-    float acc[PD] = {}, l = 0.0f;
+    for (uint32_t z = col; z < sh.live; z += 16) top = fmaxf(top, rec[z * step + HD]);
+#pragma unroll
+    for (int off = 8; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    constexpr int PD = HD / 64;  // four dims from 4 (col + 16 e) on
+    float acc[PD][4] = {}, l = 0.0f;
 #pragma unroll 4
     for (uint32_t z = 0; z < sh.live; ++z) {
         const float *rz = rec + z * step;
@@ -741,14 +822,26 @@ __global__ __launch_bounds__(4 * kWave) void rows_combine(Args a) {
         const float f = mz == top ? 1.0f : __builtin_amdgcn_exp2f((mz - top) * a.c);
         l = fmaf(lz, f, l);
 #pragma unroll
-        for (int e = 0; e < PD; ++e) acc[e] = fmaf(rz[lane + 64 * e], f, acc[e]);
+        for (int e = 0; e < PD; ++e) {
+            float v[4];
+            load_f32<F32, 4>(rz + 4 * (col + 16 * e), v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[e][i] = fmaf(v[i], f, acc[e][i]);
+        }
     }
     const uint32_t pr = t.row0 + r, tk = pr / a.group, hd = g * a.group + pr % a.group;
+    const float inv = 1.0f / l;
     const bool none = top == -__builtin_inff() && l == 0.0f;  // no attended key
+    const size_t o0 = (size_t)(t.first + tk) * a.out_stride + (size_t)hd * HD;
 #pragma unroll
-    for (int e = 0; e < PD; ++e)
-        store_elem(a.out, a.out_dtype, (size_t)(t.first + tk) * a.out_stride + (size_t)hd * HD + lane + 64 * e,
-                   none ? 0.0f : acc[e] / l);
+    for (int e = 0; e < PD; ++e) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[e][i] = none ? 0.0f : acc[e][i] * inv;
+        const size_t o = o0 + 4 * (col + 16 * e);
+        if (a.out_dtype == FELLM_DTYPE_F32) store_f32<F32, 4>(static_cast<float *>(a.out) + o, acc[e]);
+        else if (a.out_dtype == FELLM_DTYPE_F16) store_f32<F16, 4>(static_cast<_Float16 *>(a.out) + o, acc[e]);
+        else store_f32<BF16, 4>(static_cast<uint16_t *>(a.out) + o, acc[e]);
+    }
 }
 
 }  // namespace rows_attn

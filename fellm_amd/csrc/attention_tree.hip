@@ -7,6 +7,7 @@
 #include "attention_rows.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace fellm {
 namespace {
@@ -26,11 +27,15 @@ struct Plan {
 #define FELLM_TREE_GROUPS 512
 #endif
 #ifndef FELLM_TREE_MIN
-#define FELLM_TREE_MIN 128
+#define FELLM_TREE_MIN 192
 #endif
 #ifndef FELLM_TREE_MAX
 #define FELLM_TREE_MAX 2048
 #endif
+#ifndef FELLM_TREE_MANY
+#define FELLM_TREE_MANY 1024
+#endif
+constexpr uint32_t kTargetMany = FELLM_TREE_MANY;
 constexpr uint32_t kTargetGroups = FELLM_TREE_GROUPS, kMinKeys = FELLM_TREE_MIN, kMaxKeys = FELLM_TREE_MAX;
 
 Plan plan(uint32_t n_seqs, uint32_t tokens, uint32_t group, uint32_t n_kv, uint32_t max_nodes, uint32_t max_prefix) {
@@ -39,10 +44,11 @@ Plan plan(uint32_t n_seqs, uint32_t tokens, uint32_t group, uint32_t n_kv, uint3
     const uint64_t rows = (uint64_t)max_nodes * group;
     p.rw = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
     const uint32_t bm = kRows * p.rw;
-    p.tiles = (uint64_t)tokens * group / bm + n_seqs;
+    // one sequence: exactly its tiles; more: the most that tokens rows can need
+    p.tiles = n_seqs == 1 ? ((uint64_t)tokens * group + bm - 1) / bm : (uint64_t)tokens * group / bm + n_seqs;
     const uint64_t used = std::min<uint64_t>(p.tiles, (uint64_t)n_seqs * ((rows + bm - 1) / bm)) * n_kv;
     const uint64_t keys = (uint64_t)max_prefix + max_nodes;
-    uint64_t splits = std::min<uint64_t>((kTargetGroups + used - 1) / std::max<uint64_t>(used, 1), (keys + kMinKeys - 1) / kMinKeys);
+    uint64_t splits = std::min<uint64_t>(((n_seqs > 1 ? kTargetMany : kTargetGroups) + used - 1) / std::max<uint64_t>(used, 1), (keys + kMinKeys - 1) / kMinKeys);
     splits = std::max<uint64_t>(splits, n_seqs > 1 ? (keys + kMaxKeys - 1) / kMaxKeys : 1);
     if (splits == 1) {
         p.splits = 1;
@@ -60,23 +66,28 @@ uint64_t part_bytes(const Plan &p, uint32_t n_kv, uint32_t head_dim) {
     return p.splits <= 1 ? 0 : p.tiles * n_kv * p.splits * kRows * p.rw * (head_dim + 4) * 4;
 }
 
+#ifndef CFG4
+#define CFG4 64, 2, 2
+#endif
+#ifndef OCC12
+#define OCC12 2
+#endif
+#ifndef CFG4P
+#define CFG4P 32, 2, 2
+#endif
+template <int KT_, int OCC_, int NST_> struct Layout { static constexpr int KT = KT_, OCC = OCC_, NST = NST_; };
 template <typename E, int HD, int RW, bool PARTS>
 int launch_tree(const Plan &p, const Args &a, hipStream_t st) {
     constexpr int KW = RW == 4 ? 1 : HD == 256 || RW == 2 ? 2 : 4;
-    #ifndef TKT
-#define TKT 64
-#define TOCC 2
-#endif
-    constexpr int KT = RW == 4 && HD != 256 && !(PARTS && HD == 128) ? (HD == 128 ? TKT : 64) : 32;
-    constexpr int OCC = RW == 4 && HD <= 128 && !PARTS ? (HD == 128 ? TOCC : 2) : 1;
+    using L = std::conditional_t<RW == 4 && HD != 256, std::conditional_t<PARTS, Layout<CFG4P>, Layout<CFG4>>, Layout<32, HD == 256 || (RW == 1 && HD == 128) ? 1 : OCC12, 2>>;
     constexpr uint32_t BM = kRows * RW;
-    const uint64_t grid = p.tiles * a.n_kv * a.splits;
+    const uint64_t grid = p.tiles * a.n_kv * a.splits, join = p.tiles * a.n_kv * (BM / kJoinRows);
     // a launch has fewer than 2^32 threads
-    if (std::max(grid, p.tiles * a.n_kv * (BM / 4)) > 0xffffffffull / (4 * kWave)) return FELLM_ERR_SHAPE;
-    FELLM_LAUNCH((rows_kernel<E, HD, RW, KW, KT, true, PARTS, OCC>), dim3((uint32_t)grid), dim3(kWave * RW * KW), 0, st, a);
+    if (std::max(grid, join) > 0xffffffffull / (4 * kWave)) return FELLM_ERR_SHAPE;
+    FELLM_LAUNCH((rows_kernel<E, HD, RW, KW, L::KT, true, PARTS, L::OCC, L::NST>), dim3((uint32_t)grid), dim3(kWave * RW * KW), 0, st, a);
     int rc = launch_status();
     if (rc != FELLM_OK || a.splits == 1) return rc;
-    FELLM_LAUNCH((rows_combine<HD, BM>), dim3((uint32_t)(p.tiles * a.n_kv * (BM / 4))), dim3(4 * kWave), 0, st, a);
+    FELLM_LAUNCH((rows_combine<HD, BM>), dim3((uint32_t)join), dim3(kJoinRows * 16), 0, st, a);
     return launch_status();
 }
 
