@@ -87,11 +87,10 @@ extern "C" int fellm_rocm_prompt_attention(const void *q, uint32_t q_stride, con
     a.n_heads = n_heads;
     a.n_kv = n_kv_heads;
     a.group = n_heads / n_kv_heads;
+    a.by_group = rows_attn::Divisor(a.group);
     a.c = scale * 1.4426950408889634f;
     a.causal = causal;
     a.window = window;
-    a.splits = 1;
-    a.keys_per_split = 0x7fffffc0u;
     hipStream_t st = as_stream(stream);
     return dtype == FELLM_DTYPE_BF16 ? prompt_heads<rows_attn::ElemBF16>(head_dim, a, st)
                                      : prompt_heads<rows_attn::ElemF16>(head_dim, a, st);

@@ -82,6 +82,24 @@ struct ElemBF16 {
     }
 };
 
+// Division by a number fixed at the launch, by a multiplication with its
+// rounded-up reciprocal (Granlund and Montgomery, 1994).
+struct Divisor {
+    uint32_t d, m, s1, s2;
+    Divisor() = default;
+    explicit Divisor(uint32_t n) : d(n) {
+        uint32_t l = 0;
+        while (l < 32 && (1ull << l) < n) ++l;
+        m = (uint32_t)((((1ull << l) - n) << 32) / n + 1);
+        s1 = l < 1 ? l : 1;
+        s2 = l < 1 ? 0 : l - 1;
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t x) const {
+        const uint32_t t = __umulhi(m, x);
+        return (t + ((x - t) >> s1)) >> s2;
+    }
+};
+
 struct Args {
     const void *q;
     void *out;
@@ -92,6 +110,7 @@ struct Args {
     const uint32_t *before; // [n_seqs] cached keys before a sequence's first token, or null
     const uint32_t *mask;   // [tokens, mask_words] bits of the sequence's own tokens, or null
     uint32_t mask_words, n_seqs, tokens, n_heads, n_kv, group;
+    Divisor by_group;
     float c;                // scale log2 e
     uint32_t causal, window;
     uint32_t max_before;    // bound that `before` is clamped to
@@ -100,8 +119,9 @@ struct Args {
     uint64_t arena_len, block_bytes, n_table;
     const uint32_t *table;
     uint32_t n_logical, n_layers, layer, stride;
-    // split of the keys
-    uint32_t splits, keys_per_split;
+    // the launch's share of the rounds of keys (paged): at least this many a
+    // workgroup, the records of tiles that several share (null: whole tiles)
+    uint32_t min_rounds;
     float *part;
 };
 
@@ -390,25 +410,128 @@ __device__ __forceinline__ void store_tile(typename O::T *to, const f32x16 &v, u
 template <int HD>
 constexpr uint32_t kRec = HD + 4;
 
-// Keys of a tile of rows, and the part of them that split z has.
-struct Share {
-    uint32_t begin, end;  // first a multiple of 64
-    uint32_t live;        // splits with keys (0: no keys at all)
+// Keys of a tile of rows: [begin, end), begin a multiple of 64.
+struct Keys {
+    uint32_t begin, end;
 };
 template <uint32_t BM>
-__device__ __forceinline__ Share key_share(const Args &a, const Tile &t, uint32_t z) {
-    const uint32_t i0 = t.row0 / a.group, i1 = min(t.n, (t.row0 + BM - 1) / a.group + 1);
-    const KeyRange f = row_keys(a, t, i0), e = row_keys(a, t, i1 - 1);
-    uint32_t lo = f.lo / 64 * 64, hi = e.hi;
-    Share s;
-    const uint32_t total = hi > lo ? hi - lo : 0;
-    const uint32_t live = (total + a.keys_per_split - 1) / a.keys_per_split;
-    s.live = min(live, a.splits);
-    s.begin = lo + z * a.keys_per_split;
-    // the last split takes what is past the launch's bound on the keys
-    s.end = z + 1 >= s.live ? hi : min(hi, s.begin + a.keys_per_split);
-    return s;
+__device__ __forceinline__ Keys tile_keys(const Args &a, const Tile &t) {
+    const uint32_t i0 = a.by_group(t.row0), i1 = min(t.n, a.by_group(t.row0 + BM - 1) + 1);
+    return Keys{row_keys(a, t, i0).lo / 64 * 64, row_keys(a, t, i1 - 1).hi};
 }
+
+// Inclusive sum over the wavefront's lanes.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, true);  // row_shr:1, 2, 4, 8
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, true);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, true);
+    const uint32_t a = __builtin_amdgcn_readlane(v, 15), b = a + __builtin_amdgcn_readlane(v, 31),
+                   c = b + __builtin_amdgcn_readlane(v, 47), row = threadIdx.x % kWave / 16;
+    return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
+}
+
+// How a paged launch shares its work.  The rounds of TK keys of every tile, tiles
+// in the order of the sequences, are one line for each K/V head, which the head's
+// `ids` workgroups cut into pieces, so that sequences of any lengths keep every
+// workgroup busy and all of them are resident at once.  Where there are
+// workgroups enough a piece is a part of one tile (per > 1 rounds, share 1);
+// else the line is cut into equal shares, and a workgroup walks the tiles that
+// its share touches, of which the first and the last can be shared with others:
+// two records.  (Measured against tiles cut at fixed numbers of keys: 32 trees of
+// up to 32 tokens behind 616 .. 8192 keys, 64/8 heads of 128, bf16, 124 and 118
+// us; 16 drafted tokens behind 32768 keys, 16/4 heads of 256, 125 and 58.)
+// Lane b holds sequence c + b.
+template <uint32_t BM, uint32_t TK>
+struct Line {
+    const Args &a;
+    struct Lane {
+        uint32_t first, n, before, tiles, rounds;  // rounds of each tile
+    } l0;
+    uint32_t per, share;  // rounds of a unit of the line, units of a workgroup
+    uint32_t units;       // of the line
+
+    __device__ __forceinline__ Line(const Args &args, uint32_t ids) : a(args) {
+        l0 = lane(0);
+        per = 1;
+        units = total();
+        share = (units + ids - 1) / ids;
+        if (a.part) {
+            per = share = max(share, a.min_rounds);
+            uint32_t pieces = total();
+            if (pieces > ids) {
+                // two rounds more than an equal share cost less than a second
+                // tile's start (about five)
+                per = share + 2;
+                pieces = total();
+            }
+            if (pieces <= ids) share = 1, units = pieces;
+            else per = 1;
+        }
+    }
+    __device__ __forceinline__ Lane lane(uint32_t c) const {
+        const uint32_t b = c + threadIdx.x % kWave;
+        Lane l{0, 0, 0, 0, 1};
+        if (b < a.n_seqs) {
+            l.first = min(a.cu[b], a.tokens);
+            const uint32_t end = min(a.cu[b + 1], a.tokens);
+            l.n = end > l.first ? end - l.first : 0;
+            l.before = min(a.before[b], a.max_before);
+        }
+        l.tiles = (l.n * a.group + BM - 1) / BM;
+        if (a.part && l.n) {
+            uint32_t keys = l.before + l.n;
+            // the last keys of the tile's first token, its other tokens, the alignment
+            if (a.window) keys = min(keys, min(a.window, 1u << 30) + BM + 63);
+            l.rounds = (keys + TK - 1) / TK;
+        }
+        return l;
+    }
+    __device__ __forceinline__ uint32_t units_of(const Lane &l) const {
+        return per == 1 ? l.rounds : (l.rounds + per - 1) / per;
+    }
+    __device__ __forceinline__ uint32_t total() const {
+        const uint32_t here = l0.tiles * units_of(l0);
+        if (a.n_seqs == 1) return __builtin_amdgcn_readfirstlane(here);
+        uint32_t sum = wave_total(here);
+        for (uint32_t c = kWave; c < a.n_seqs; c += kWave) {
+            const Lane l = lane(c);
+            sum += wave_total(l.tiles * units_of(l));
+        }
+        return sum;
+    }
+    struct Spot {
+        Tile t;
+        uint32_t rounds, units, at;  // of the tile, and where it begins on the line
+    };
+    // BY_TILE: tile number x; else the tile that holds unit x.  n = 0: none.
+    template <bool BY_TILE>
+    __device__ __forceinline__ Spot find(uint32_t x) const {
+        Spot s{Tile{0, 0, 0, 0, 0}, 1, 1, 0};
+        uint32_t tiles = 0, at = 0;
+        for (uint32_t c = 0; c < a.n_seqs; c += kWave) {
+            const Lane l = c ? lane(c) : l0;
+            const uint32_t u = units_of(l), v = l.tiles * u;
+            const bool one = a.n_seqs == 1;
+            const uint32_t vi = one ? v : wave_scan(v), ti = !BY_TILE ? 0 : one ? l.tiles : wave_scan(l.tiles);
+            const uint64_t past = __ballot((BY_TILE ? tiles + ti : at + vi) > x);
+            if (past) {
+                const uint32_t b = (uint32_t)__builtin_ctzll(past);
+                auto of = [&](uint32_t value) { return (uint32_t)__builtin_amdgcn_readlane(value, b); };
+                const uint32_t begin = at + of(vi - v);
+                s.rounds = of(l.rounds);
+                s.units = of(u);
+                const uint32_t k = BY_TILE ? x - (tiles + of(ti - l.tiles)) : (x - begin) / s.units;
+                s.t = Tile{c + b, k * BM, of(l.first), of(l.n), of(l.before)};
+                s.at = begin + k * s.units;
+                return s;
+            }
+            if (BY_TILE) tiles += __builtin_amdgcn_readlane(ti, kWave - 1);
+            at += __builtin_amdgcn_readlane(vi, kWave - 1);
+        }
+        return s;
+    }
+};
 
 // A buffer resource in scalar registers: everything it is made of is the same in
 // all lanes, but where the compiler does not see that it would loop over lanes
@@ -447,25 +570,54 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     const uint32_t lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const uint32_t rw = wave % RW, kw = wave / RW;
     const uint32_t n = lane % 32, h = lane / 32;
-    // Neighbouring workgroups take the K/V heads in turn (one XCD sees few of
-    // them), the tiles with most keys first.
-    const uint32_t per = gridDim.x / a.splits;
-    const uint32_t z = blockIdx.x / per, id = blockIdx.x % per;
-    const uint32_t g = id % a.n_kv, tiles = per / a.n_kv;
-    const uint32_t ti = id / a.n_kv;
-    const Tile t = tile_of<BM>(a, ti, tiles);
-    if (t.n == 0) return;
-    const Share sh = key_share<BM>(a, t, z);
-    if (z >= max(sh.live, 1u)) return;
+    // Neighbouring workgroups take the K/V heads in turn (one XCD sees few of them).
+    const uint32_t g = blockIdx.x % a.n_kv, id = blockIdx.x / a.n_kv, ids = gridDim.x / a.n_kv;
+    // this workgroup's piece [x, x_end) of the line (contiguous K/V: its one tile)
+    const auto line = [&] {
+        if constexpr (PAGED) return Line<BM, TK>(a, ids);
+        else return 0;
+    }();
+    uint32_t x = 0, x_end = 1;
+    if constexpr (PAGED) {
+        if ((uint64_t)id * line.share >= line.units) return;
+        x = id * line.share;
+        x_end = min(line.units, x + line.share);
+    }
+    for (uint32_t again = 0; x < x_end; again = 1) {
+    Tile t;
+    Keys sh;
+    bool direct = true;
+    float *part = nullptr;  // the tile's records where others share it
+    if constexpr (PAGED) {
+        const auto spot = line.template find<false>(x);
+        t = spot.t;
+        if (t.n == 0) break;  // offsets that are none: nothing more to find
+        sh = tile_keys<BM>(a, t);
+        const uint32_t u0 = x - spot.at, u1 = min(spot.units, u0 + x_end - x);
+        direct = u1 - u0 == spot.units;
+        if (!direct) {
+            part = a.part + (size_t)(2 * (g * ids + id) + again) * BM * kRec<HD>;
+            const uint32_t lo = sh.begin;
+            sh.begin = lo + u0 * line.per * TK;
+            if (u1 < spot.units) sh.end = min(sh.end, lo + u1 * line.per * TK);
+        }
+        x += u1 - u0;
+        if (again) __syncthreads();  // the buffers may still be read for the tile before
+    } else {
+        t = tile_of<BM>(a, id, ids);
+        if (t.n == 0) return;
+        sh = tile_keys<BM>(a, t);
+        ++x;
+    }
 
     const uint32_t row = t.row0 + rw * kRows + n;
     const bool valid = row < t.n * a.group;
     const uint32_t rrow = valid ? row : t.n * a.group - 1;
-    const uint32_t token = rrow / a.group, head = g * a.group + rrow % a.group;
+    const uint32_t token = a.by_group(rrow), head = g * a.group + rrow - token * a.group;
     const KeyRange mine = row_keys(a, t, token);
     // keys that every row of this wavefront attends, and that any does
     const uint32_t w0 = min(t.row0 + rw * kRows, t.n * a.group - 1), w1 = min(w0 + kRows - 1, t.n * a.group - 1);
-    const KeyRange rf = row_keys(a, t, w0 / a.group), rl = row_keys(a, t, w1 / a.group);
+    const KeyRange rf = row_keys(a, t, a.by_group(w0)), rl = row_keys(a, t, a.by_group(w1));
     const uint32_t full_lo = rl.lo, full_hi = a.mask ? t.before : rf.hi, any_lo = rf.lo, any_hi = rl.hi;
 
     f32x16 acc[ND];
@@ -737,17 +889,13 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     }
 
     // ---- results
-    const bool direct = sh.live <= 1;
-    auto record = [&](uint32_t r) {  // of packed row r of the tile
-        return a.part + (((size_t)ti * a.n_kv + g) * a.splits + z) * BM * kRec<HD> + (size_t)r * kRec<HD>;
-    };
     const bool bad = valid && some && !(probe == 0.0f && l > 0.0f);
     // exchanges between a row's two lanes follow: both take part or neither, as
     // valid and bad are the row's
     if (valid && !bad) {
         const float inv = !direct ? 1.0f : some ? 1.0f / l : 0.0f;
         const size_t o0 = (size_t)(t.first + token) * a.out_stride + (size_t)head * HD;
-        float *rec = record(rw * kRows + n);
+        float *rec = part + (size_t)(rw * kRows + n) * kRec<HD>;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             if (KW > 1 && d % KW != (int)kw) continue;
@@ -773,16 +921,15 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
             rec[HD + 1] = l;
         }
     }
-    if (kw) return;
-    uint64_t again = __ballot(bad) & 0xffffffffull;
-    while (again) {
-        const uint32_t r = (uint32_t)__builtin_ctzll(again);
-        again &= again - 1;
-        const uint32_t pr = t.row0 + rw * kRows + r, tk = pr / a.group, hd = g * a.group + pr % a.group;
+    uint64_t redo = kw ? 0 : __ballot(bad) & 0xffffffffull;
+    while (redo) {
+        const uint32_t r = (uint32_t)__builtin_ctzll(redo);
+        redo &= redo - 1;
+        const uint32_t pr = t.row0 + rw * kRows + r, tk = a.by_group(pr), hd = g * a.group + pr - tk * a.group;
         float sums[HD / 64], m1, l1;
         careful_row<E, HD, PAGED>(a, t, g, tk, hd, sh.begin, sh.end, kBias, sums, m1, l1);
         const bool none = m1 == -__builtin_inff() && l1 == 0.0f;  // no attended key
-        float *rec = record(rw * kRows + r);
+        float *rec = part + (size_t)(rw * kRows + r) * kRec<HD>;
 #pragma unroll
         for (int e = 0; e < HD / 64; ++e) {
             if (direct)
@@ -795,29 +942,39 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
             rec[HD + 1] = l1;
         }
     }
+    }
 }
 
-// Joins the splits' records: 16 lanes a row, 16 rows a workgroup.
-constexpr uint32_t kJoinRows = 16;
-template <int HD, uint32_t BM>
-__global__ __launch_bounds__(kJoinRows * 16) void rows_combine(Args a) {
-    const uint32_t id = blockIdx.x / (BM / kJoinRows), g = id % a.n_kv, ti = id / a.n_kv;
-    const uint32_t r = blockIdx.x % (BM / kJoinRows) * kJoinRows + threadIdx.x / 16, col = threadIdx.x % 16;
-    const Tile t = tile_of<BM>(a, ti, gridDim.x / (BM / kJoinRows) / a.n_kv);
-    if (t.n == 0 || t.row0 + r >= t.n * a.group) return;
-    const Share sh = key_share<BM>(a, t, 0);
-    if (sh.live <= 1) return;
-    const float *rec = a.part + ((size_t)ti * a.n_kv + g) * a.splits * BM * kRec<HD> + (size_t)r * kRec<HD>;
-    const size_t step = (size_t)BM * kRec<HD>;
+// Joins the records of tiles that several workgroups shared: 16 lanes a row read
+// one record, Q groups of 16 lanes every Q-th.  ids: the workgroups per K/V head
+// of the launch before.
+constexpr uint32_t kJoinThreads = 256;
+template <int HD, uint32_t BM, uint32_t TK, int Q>
+__global__ __launch_bounds__(kJoinThreads) void rows_combine(Args a, uint32_t ids) {
+    constexpr uint32_t ROWS = kJoinThreads / 16 / Q;  // of a workgroup
+    const uint32_t id = blockIdx.x / (BM / ROWS), g = id % a.n_kv;
+    const uint32_t r = blockIdx.x % (BM / ROWS) * ROWS + threadIdx.x / (16 * Q);
+    const uint32_t col = threadIdx.x % 16, part = threadIdx.x / 16 % Q;
+    const Line<BM, TK> line(a, ids);
+    const auto spot = line.template find<true>(id / a.n_kv);
+    const Tile t = spot.t;
+    if (t.n == 0 || spot.units == 1 || t.row0 + r >= t.n * a.group) return;
+    const uint32_t w0 = spot.at / line.share, w1 = (spot.at + spot.units - 1) / line.share;
+    if (w0 == w1) return;
+    // Workgroup w's first record if its piece begins inside the tile or with it, else its second.
+    auto record = [&](uint32_t w) {
+        const uint32_t slot = 2 * (g * ids + w) + (w * line.share >= spot.at ? 0 : 1);
+        return a.part + ((size_t)slot * BM + r) * kRec<HD>;
+    };
     float top = -__builtin_inff();
-    for (uint32_t z = col; z < sh.live; z += 16) top = fmaxf(top, rec[z * step + HD]);
+    for (uint32_t w = w0 + col + 16 * part; w <= w1; w += 16 * Q) top = fmaxf(top, record(w)[HD]);
 #pragma unroll
-    for (int off = 8; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
+    for (int off = 8 * Q; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
     constexpr int PD = HD / 64;  // four dims from 4 (col + 16 e) on
     float acc[PD][4] = {}, l = 0.0f;
 #pragma unroll 4
-    for (uint32_t z = 0; z < sh.live; ++z) {
-        const float *rz = rec + z * step;
+    for (uint32_t w = w0 + part; w <= w1; w += Q) {
+        const float *rz = record(w);
         const float mz = rz[HD], lz = rz[HD + 1];
         const float f = mz == top ? 1.0f : __builtin_amdgcn_exp2f((mz - top) * a.c);
         l = fmaf(lz, f, l);
@@ -829,7 +986,16 @@ __global__ __launch_bounds__(kJoinRows * 16) void rows_combine(Args a) {
             for (int i = 0; i < 4; ++i) acc[e][i] = fmaf(v[i], f, acc[e][i]);
         }
     }
-    const uint32_t pr = t.row0 + r, tk = pr / a.group, hd = g * a.group + pr % a.group;
+#pragma unroll
+    for (int off = 16; off < 16 * Q; off <<= 1) {
+        l += __shfl_xor(l, off);
+#pragma unroll
+        for (int e = 0; e < PD; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[e][i] += __shfl_xor(acc[e][i], off);
+    }
+    if (part) return;
+    const uint32_t pr = t.row0 + r, tk = a.by_group(pr), hd = g * a.group + pr - tk * a.group;
     const float inv = 1.0f / l;
     const bool none = top == -__builtin_inff() && l == 0.0f;  // no attended key
     const size_t o0 = (size_t)(t.first + tk) * a.out_stride + (size_t)hd * HD;

@@ -13,95 +13,76 @@ namespace fellm {
 namespace {
 using namespace rows_attn;
 
-struct Plan {
-    uint32_t rw;  // wavefronts that own rows: tiles of 32 rw rows
-    uint64_t tiles;
-    uint32_t splits, keys_per_split;
+// Layouts by the rows of a sequence: tiles of 32, 64 or 128 rows, the smallest
+// that holds them; the wavefronts without rows of their own share the keys.
+// KW: those wavefronts; KT: keys of a wavefront's tile; OCC: wavefronts per SIMD.
+template <int HD, int RW, bool PARTS>
+struct Layout {
+    static constexpr int KW = RW == 4 ? 1 : HD == 256 || RW == 2 ? 2 : 4;
+    static constexpr int KT = RW == 4 && HD != 256 && !PARTS ? 64 : 32;
+    static constexpr int OCC = HD == 256 || (RW == 1 && HD == 128) ? 1 : 2;
+    static constexpr uint32_t BM = kRows * RW, TK = KT * KW;
+    // Workgroups that are resident at once, and the least keys that one takes.
+    static constexpr uint32_t kSlots = 256 * OCC, kMinRounds = (192 + TK - 1) / TK;
 };
 
-// Tiles of 32, 64 or 128 rows, the smallest that holds a sequence's rows: the
-// wavefronts without rows of their own share the keys.  The keys are split until
-// the launch has kTargetGroups workgroups, in parts of at least kMinKeys; the
-// keys of several sequences, whose lengths differ, in parts of at most kMaxKeys.
-#ifndef FELLM_TREE_GROUPS
-#define FELLM_TREE_GROUPS 512
-#endif
-#ifndef FELLM_TREE_MIN
-#define FELLM_TREE_MIN 192
-#endif
-#ifndef FELLM_TREE_MAX
-#define FELLM_TREE_MAX 2048
-#endif
-#ifndef FELLM_TREE_MANY
-#define FELLM_TREE_MANY 1024
-#endif
-constexpr uint32_t kTargetMany = FELLM_TREE_MANY;
-constexpr uint32_t kTargetGroups = FELLM_TREE_GROUPS, kMinKeys = FELLM_TREE_MIN, kMaxKeys = FELLM_TREE_MAX;
+struct Plan {
+    uint64_t tiles;       // of all sequences, at most
+    uint32_t ids;         // workgroups per K/V head
+    uint64_t part_bytes;  // their records
+};
 
+template <int HD, int RW, bool PARTS>
 Plan plan(uint32_t n_seqs, uint32_t tokens, uint32_t group, uint32_t n_kv, uint32_t max_nodes, uint32_t max_prefix) {
+    using L = Layout<HD, RW, PARTS>;
     Plan p;
-    max_nodes = std::min(std::max(max_nodes, 1u), tokens);
-    const uint64_t rows = (uint64_t)max_nodes * group;
-    p.rw = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
-    const uint32_t bm = kRows * p.rw;
     // one sequence: exactly its tiles; more: the most that tokens rows can need
-    p.tiles = n_seqs == 1 ? ((uint64_t)tokens * group + bm - 1) / bm : (uint64_t)tokens * group / bm + n_seqs;
-    const uint64_t used = std::min<uint64_t>(p.tiles, (uint64_t)n_seqs * ((rows + bm - 1) / bm)) * n_kv;
-    const uint64_t keys = (uint64_t)max_prefix + max_nodes;
-    uint64_t splits = std::min<uint64_t>(((n_seqs > 1 ? kTargetMany : kTargetGroups) + used - 1) / std::max<uint64_t>(used, 1), (keys + kMinKeys - 1) / kMinKeys);
-    splits = std::max<uint64_t>(splits, n_seqs > 1 ? (keys + kMaxKeys - 1) / kMaxKeys : 1);
-    if (splits == 1) {
-        p.splits = 1;
-        p.keys_per_split = 0x7fffffc0u;
-        return p;
-    }
-    p.keys_per_split = (uint32_t)(((keys + splits - 1) / splits + 63) / 64 * 64);
-    p.splits = (uint32_t)((keys + p.keys_per_split - 1) / p.keys_per_split);
-    // a share starts at a multiple of 64 below its first key
-    if (p.splits == 1) p.keys_per_split = 0x7fffffc0u;
+    const uint64_t all = (uint64_t)tokens * group;
+    p.tiles = n_seqs == 1 ? (all + L::BM - 1) / L::BM : all / L::BM + n_seqs;
+    const uint64_t used = std::min<uint64_t>(p.tiles, (uint64_t)n_seqs * (((uint64_t)max_nodes * group + L::BM - 1) / L::BM));
+    const uint64_t rounds = used * (((uint64_t)max_prefix + max_nodes + L::TK - 1) / L::TK);
+    const uint64_t most = std::max<uint64_t>((rounds + L::kMinRounds - 1) / L::kMinRounds + used, 1);
+    p.ids = (uint32_t)std::min<uint64_t>(std::max(L::kSlots / n_kv, 1u), most);
+    p.part_bytes = p.ids == 1 ? 0 : (uint64_t)p.ids * n_kv * 2 * L::BM * kRec<HD> * 4;
     return p;
 }
 
-uint64_t part_bytes(const Plan &p, uint32_t n_kv, uint32_t head_dim) {
-    return p.splits <= 1 ? 0 : p.tiles * n_kv * p.splits * kRows * p.rw * (head_dim + 4) * 4;
+template <typename Fn>
+auto with_layout(uint32_t head_dim, uint64_t rows, bool parts, Fn &&f) {
+    auto pick_rows = [&]<int HD, bool PARTS>() {
+        if (rows <= 32) return f.template operator()<HD, 1, PARTS>();
+        if (rows <= 64) return f.template operator()<HD, 2, PARTS>();
+        return f.template operator()<HD, 4, PARTS>();
+    };
+    auto pick_head = [&]<bool PARTS>() {
+        if (head_dim == 64) return pick_rows.template operator()<64, PARTS>();
+        if (head_dim == 128) return pick_rows.template operator()<128, PARTS>();
+        return pick_rows.template operator()<256, PARTS>();
+    };
+    return parts ? pick_head.template operator()<true>() : pick_head.template operator()<false>();
 }
 
-#ifndef CFG4
-#define CFG4 64, 2, 2
-#endif
-#ifndef OCC12
-#define OCC12 2
-#endif
-#ifndef CFG4P
-#define CFG4P 32, 2, 2
-#endif
-template <int KT_, int OCC_, int NST_> struct Layout { static constexpr int KT = KT_, OCC = OCC_, NST = NST_; };
 template <typename E, int HD, int RW, bool PARTS>
-int launch_tree(const Plan &p, const Args &a, hipStream_t st) {
-    constexpr int KW = RW == 4 ? 1 : HD == 256 || RW == 2 ? 2 : 4;
-    using L = std::conditional_t<RW == 4 && HD != 256, std::conditional_t<PARTS, Layout<CFG4P>, Layout<CFG4>>, Layout<32, HD == 256 || (RW == 1 && HD == 128) ? 1 : OCC12, 2>>;
-    constexpr uint32_t BM = kRows * RW;
-    const uint64_t grid = p.tiles * a.n_kv * a.splits, join = p.tiles * a.n_kv * (BM / kJoinRows);
-    // a launch has fewer than 2^32 threads
-    if (std::max(grid, join) > 0xffffffffull / (4 * kWave)) return FELLM_ERR_SHAPE;
-    FELLM_LAUNCH((rows_kernel<E, HD, RW, KW, L::KT, true, PARTS, L::OCC, L::NST>), dim3((uint32_t)grid), dim3(kWave * RW * KW), 0, st, a);
+int launch_tree(const Plan &p, Args a, hipStream_t st) {
+    using L = Layout<HD, RW, PARTS>;
+    const uint64_t grid = (uint64_t)p.ids * a.n_kv, rows = p.tiles * a.n_kv * L::BM;
+    // a launch has fewer than 2^32 threads; positions on the line are 32 bits
+    if (std::max(grid * 4 * kWave, rows * 64) > 0xffffffffull) return FELLM_ERR_SHAPE;
+    if (p.tiles * (((uint64_t)a.max_before + a.tokens) / L::TK + 1) > 0x3fffffffull) return FELLM_ERR_SHAPE;
+    a.min_rounds = L::kMinRounds;
+    FELLM_LAUNCH((rows_kernel<E, HD, RW, L::KW, L::KT, true, PARTS, L::OCC>), dim3((uint32_t)grid),
+                 dim3(kWave * RW * L::KW), 0, st, a);
     int rc = launch_status();
-    if (rc != FELLM_OK || a.splits == 1) return rc;
-    FELLM_LAUNCH((rows_combine<HD, BM>), dim3((uint32_t)join), dim3(kJoinRows * 16), 0, st, a);
+    if (rc != FELLM_OK || !a.part) return rc;
+    // 64 lanes a row where a tile can have many records (one sequence of 32768
+    // keys, 28/4 heads: 44.0 -> 38.1 us; eight of up to 1000 the other way 22.5, 24.6)
+    auto join = [&]<int Q>() {
+        FELLM_LAUNCH((rows_combine<HD, L::BM, L::TK, Q>), dim3((uint32_t)(rows / (kJoinThreads / 16 / Q))),
+                     dim3(kJoinThreads), 0, st, a, p.ids);
+    };
+    if (p.ids > 4 * p.tiles) join.template operator()<4>();
+    else join.template operator()<1>();
     return launch_status();
-}
-
-template <typename E, int HD, bool PARTS>
-int tree_rows(const Plan &p, const Args &a, hipStream_t st) {
-    return p.rw == 1 ? launch_tree<E, HD, 1, PARTS>(p, a, st)
-                     : p.rw == 2 ? launch_tree<E, HD, 2, PARTS>(p, a, st) : launch_tree<E, HD, 4, PARTS>(p, a, st);
-}
-
-template <typename E, bool PARTS>
-int tree_heads(uint32_t head_dim, const Plan &p, const Args &a, hipStream_t st) {
-    if (head_dim == 64) return tree_rows<E, 64, PARTS>(p, a, st);
-    if (head_dim == 128) return tree_rows<E, 128, PARTS>(p, a, st);
-    return tree_rows<E, 256, PARTS>(p, a, st);
 }
 
 bool tree_heads_ok(uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim) {
@@ -116,8 +97,13 @@ extern "C" uint64_t fellm_rocm_paged_tree_attention_workspace(uint32_t n_seqs, u
                                                               uint32_t max_nodes, uint32_t max_prefix) {
     using namespace fellm;
     if (!tree_heads_ok(n_heads, n_kv_heads, head_dim) || !n_seqs || !tokens) return 0;
-    const Plan p = plan(n_seqs, tokens, n_heads / n_kv_heads, n_kv_heads, max_nodes, max_prefix);
-    return part_bytes(p, n_kv_heads, head_dim);
+    const uint32_t group = n_heads / n_kv_heads, nodes = std::min(std::max(max_nodes, 1u), tokens);
+    uint64_t need = 0;
+    for (bool parts : {false, true})
+        need = std::max(need, with_layout(head_dim, (uint64_t)nodes * group, parts, [&]<int HD, int RW, bool PARTS>() {
+                            return plan<HD, RW, PARTS>(n_seqs, tokens, group, n_kv_heads, nodes, max_prefix).part_bytes;
+                        }));
+    return need;
 }
 
 extern "C" int fellm_rocm_paged_tree_attention(const void *q, uint32_t q_dtype, void *out, uint32_t out_dtype,
@@ -160,6 +146,7 @@ extern "C" int fellm_rocm_paged_tree_attention(const void *q, uint32_t q_dtype, 
     a.n_heads = n_heads;
     a.n_kv = n_kv_heads;
     a.group = n_heads / n_kv_heads;
+    a.by_group = rows_attn::Divisor(a.group);
     a.c = scale * 1.4426950408889634f;
     a.causal = 1;
     a.window = window;
@@ -172,19 +159,13 @@ extern "C" int fellm_rocm_paged_tree_attention(const void *q, uint32_t q_dtype, 
     a.n_layers = kv->n_layers;
     a.layer = kv->layer;
     a.stride = kv->stride;
-    Plan p = plan(n_seqs, tokens, a.group, n_kv_heads, max_nodes, max_prefix);
-    if (p.splits > 1 && (!workspace || workspace_bytes < part_bytes(p, n_kv_heads, head_dim))) {
-        p.splits = 1;
-        p.keys_per_split = 0x7fffffc0u;
-    }
-    a.splits = p.splits;
-    a.keys_per_split = p.keys_per_split;
-    a.part = workspace;
     hipStream_t st = as_stream(stream);
     const bool parts = q_dtype != kv->kv_dtype || out_dtype != kv->kv_dtype;
-    if (kv->kv_dtype == FELLM_DTYPE_BF16)
-        return parts ? tree_heads<rows_attn::ElemBF16, true>(head_dim, p, a, st)
-                     : tree_heads<rows_attn::ElemBF16, false>(head_dim, p, a, st);
-    return parts ? tree_heads<rows_attn::ElemF16, true>(head_dim, p, a, st)
-                 : tree_heads<rows_attn::ElemF16, false>(head_dim, p, a, st);
+    const uint32_t nodes = std::min(std::max(max_nodes, 1u), tokens);
+    return with_layout(head_dim, (uint64_t)nodes * a.group, parts, [&]<int HD, int RW, bool PARTS>() {
+        const Plan p = plan<HD, RW, PARTS>(n_seqs, tokens, a.group, n_kv_heads, nodes, max_prefix);
+        a.part = p.part_bytes && workspace && workspace_bytes >= p.part_bytes ? workspace : nullptr;
+        return kv->kv_dtype == FELLM_DTYPE_BF16 ? launch_tree<rows_attn::ElemBF16, HD, RW, PARTS>(p, a, st)
+                                                : launch_tree<rows_attn::ElemF16, HD, RW, PARTS>(p, a, st);
+    });
 }

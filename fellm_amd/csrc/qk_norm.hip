@@ -74,12 +74,31 @@ __device__ __forceinline__ uint32_t row_position(const NormArgs &a, uint32_t row
 constexpr uint32_t kNormThreads = 256;
 constexpr uint64_t kMaxGroups = 0xffffffffull / kNormThreads;  // a launch has fewer than 2^32 threads
 
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+// V outputs, rounded by the hardware's conversion and stored in one access.
+template <typename A, bool STREAM, int V>
+__device__ __forceinline__ void put_row(typename A::T *p, const float (&v)[V]) {
+    Pack<typename A::T, V> pk;
+#pragma unroll
+    for (int i = 0; i < V; ++i) pk.v[i] = HwStore<A>::type::store(v[i]);
+    if constexpr (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, pk), reinterpret_cast<u32x4_t *>(p));
+    else store_f32<A, V>(p, v);
+}
+
 // A: activations, C: cache elements, L: lanes per head, R: rows per workgroup,
-// U: heads a lane group has in flight.
-template <typename A, typename C, int L, int R, int U, bool WRITE>
+// STREAM: non-temporal rows.
+// Measured, kernel alone (32/4 heads of 128): 16384 bf16 rows out of one
+// projection 70 -> 55 us (5.5 TB/s) with the norm weights in LDS rather than in
+// registers, one head in flight per lane group and streamed rows; f32 rows gain
+// from two heads in flight, with the weights in registers (half as many as 16-bit
+// chunks need): 4000 rows 27.4 against 34.8 us; streaming gains them only what
+// the cache cannot hold (16000 rows 121 -> 114 us, 4000 rows 27.4 -> 31.9).
+template <typename A, typename C, int L, int R, bool STREAM, bool WRITE>
 __global__ __launch_bounds__(kNormThreads) void qk_norm_kernel(NormArgs a) {
     using T = typename A::T;
     constexpr int V = 16 / sizeof(T);
+    constexpr bool REG = sizeof(T) == 4;  // norm weights in registers
+    constexpr int U = REG ? 2 : 1;        // heads that a lane group has in flight
     constexpr uint32_t GROUPS = kNormThreads / L;
     extern __shared__ __align__(16) float table[];  // per row: rope_dim / 2 cos, then as many sin
     const uint32_t half = a.rope_dim / 2;
@@ -104,6 +123,8 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_kernel(NormArgs a) {
         if (ca >= off && ca - off < a.rope_dim) pair = (ca - off) / 2;
     }
 
+    if (!active) ca = cb = 0;
+
     using P = Pack<T, V>;
     P xa[U], xb[U];
     uint32_t rr[U], hh[U];
@@ -120,8 +141,13 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_kernel(NormArgs a) {
                                : h < a.n_q + a.n_k
                                    ? static_cast<const T *>(a.k) + row * a.k_stride + (h - a.n_q) * a.head_dim
                                    : static_cast<const T *>(a.v) + row * a.v_stride + (h - a.n_q - a.n_k) * a.head_dim;
-                xa[u] = *reinterpret_cast<const P *>(src + ca);
-                xb[u] = *reinterpret_cast<const P *>(src + cb);
+                if constexpr (STREAM) {
+                    xa[u] = __builtin_bit_cast(P, __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(src + ca)));
+                    xb[u] = __builtin_bit_cast(P, __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(src + cb)));
+                } else {
+                    xa[u] = *reinterpret_cast<const P *>(src + ca);
+                    xb[u] = *reinterpret_cast<const P *>(src + cb);
+                }
             } else {
 #pragma unroll
                 for (int e = 0; e < V; ++e) xa[u].v[e] = xb[u].v[e] = T{};
@@ -129,13 +155,16 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_kernel(NormArgs a) {
         }
     };
     fetch(slot0);
-    // norm weights of the lane's channels
-    float qwa[V], qwb[V], kwa[V], kwb[V];
-    if (active) {
+    [[maybe_unused]] float qwa[V], qwb[V], kwa[V], kwb[V];
+    [[maybe_unused]] float *weights = table + R * a.rope_dim;  // of q, then of k
+    if constexpr (REG) {
         load_f32<F32, V>(a.q_weight + ca, qwa);
         load_f32<F32, V>(a.q_weight + cb, qwb);
         load_f32<F32, V>(a.k_weight + ca, kwa);
         load_f32<F32, V>(a.k_weight + cb, kwb);
+    } else {
+        for (uint32_t i = threadIdx.x; i < 2 * a.head_dim; i += kNormThreads)
+            weights[i] = i < a.head_dim ? a.q_weight[i] : a.k_weight[i - a.head_dim];
     }
     for (uint32_t i = threadIdx.x; i < nrows * half; i += kNormThreads) {
         const uint32_t r = R == 1 ? 0 : i / half, e = R == 1 ? i : i % half;
@@ -168,10 +197,19 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_kernel(NormArgs a) {
 #pragma unroll
                 for (int o = L / 2; o; o >>= 1) ss += __shfl_xor(ss, o);
                 const float r = __builtin_amdgcn_rsqf(fmaf(ss, inv_d, a.eps));
+                float wa[V], wb[V];
+                if constexpr (REG) {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) wa[e] = is_q ? qwa[e] : kwa[e], wb[e] = is_q ? qwb[e] : kwb[e];
+                } else {
+                    const float *w = weights + (is_q ? 0 : a.head_dim);
+                    load_f32<F32, V>(w + ca, wa);
+                    load_f32<F32, V>(w + cb, wb);
+                }
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    ya[u][e] = ya[u][e] * r * (is_q ? qwa[e] : kwa[e]);
-                    yb[u][e] = yb[u][e] * r * (is_q ? qwb[e] : kwb[e]);
+                    ya[u][e] = ya[u][e] * r * wa[e];
+                    yb[u][e] = yb[u][e] * r * wb[e];
                 }
                 if (pair != ~0u && here) {
                     float c[V], s[V];
@@ -200,15 +238,15 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_kernel(NormArgs a) {
             if (!here) continue;
             if (is_q) {
                 T *dst = static_cast<T *>(a.q_out) + (size_t)row * a.q_out_stride + h * a.head_dim;
-                store_f32<A, V>(dst + ca, ya[u]);
-                store_f32<A, V>(dst + cb, yb[u]);
+                put_row<A, STREAM>(dst + ca, ya[u]);
+                put_row<A, STREAM>(dst + cb, yb[u]);
                 continue;
             }
             const uint32_t kh = h - a.n_q - (is_v ? a.n_k : 0);
             if (!is_v && a.k_out) {
                 T *dst = static_cast<T *>(a.k_out) + (size_t)row * a.k_out_stride + kh * a.head_dim;
-                store_f32<A, V>(dst + ca, ya[u]);
-                store_f32<A, V>(dst + cb, yb[u]);
+                put_row<A, STREAM>(dst + ca, ya[u]);
+                put_row<A, STREAM>(dst + cb, yb[u]);
             }
             if constexpr (WRITE) {
                 const uint64_t off = row_slot(a, row, true);
@@ -296,18 +334,21 @@ int launch_norm(NormArgs a, hipStream_t st) {
         FELLM_LAUNCH((qk_norm_any_kernel<A, C, WRITE>), dim3((uint32_t)grid), dim3(kNormThreads), 0, st, a);
         return launch_status();
     }
-    auto go = [&]<int L, int R, int U>() {
+    auto go = [&]<int L, int R, bool STREAM>() {
         const uint32_t groups = (a.rows + R - 1) / R;
         // few rows: a row's heads over several workgroups
         const uint32_t most = std::max(1u, all / (kNormThreads / L));
         a.head_split = groups >= 256 ? 1 : std::min(most, std::max(1u, 512 / groups));
         if ((uint64_t)groups * a.head_split > kMaxGroups) return (int)FELLM_ERR_SHAPE;
-        FELLM_LAUNCH((qk_norm_kernel<A, C, L, R, U, WRITE>), dim3(groups * a.head_split), dim3(kNormThreads),
-                     (size_t)R * a.rope_dim * sizeof(float), st, a);
+        FELLM_LAUNCH((qk_norm_kernel<A, C, L, R, STREAM, WRITE>), dim3(groups * a.head_split), dim3(kNormThreads),
+                     ((size_t)R * a.rope_dim + (V == 4 ? 0 : 2 * a.head_dim)) * sizeof(float), st, a);
         return launch_status();
     };
     auto rows = [&]<int L>() {
-        return a.rows >= 2048 ? go.template operator()<L, 4, 2>() : go.template operator()<L, 1, 2>();
+        // (rows and their outputs; 256 MB is what the last-level cache holds)
+        const bool stream = V == 8 || (uint64_t)a.rows * 2 * all * a.head_dim * 4 > (256u << 20);
+        if (a.rows < 2048) return go.template operator()<L, 1, V == 8>();
+        return stream ? go.template operator()<L, 4, true>() : go.template operator()<L, 4, V == 8>();
     };
     const uint32_t lanes = a.head_dim / (2 * V);
     if (lanes <= 4) return rows.template operator()<4>();

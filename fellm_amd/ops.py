@@ -41,38 +41,34 @@ def _dev(*ts: torch.Tensor | None) -> None:
             raise ValueError("fellm_amd ops need contiguous tensors")
 
 
-def _rows(t: torch.Tensor, width: int | None = None) -> int:
-    """Row stride of a device matrix ``[rows, width]`` with dense rows, such as
-    a column slice of a projection's output."""
-    if not t.is_cuda:
-        raise ValueError("fellm_amd ops need device tensors (no CPU fallback)")
-    if t.dim() != 2 or (width is not None and t.shape[1] != width):
-        raise ValueError(f"expected a [rows, {width or 'width'}] tensor, got {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise ValueError("rows must be dense")
-    if t.shape[0] <= 1:
-        return t.shape[1]
-    if t.stride(0) < t.shape[1]:
-        raise ValueError("rows must not overlap")
-    return t.stride(0)
+def _here(*ts: torch.Tensor | None) -> None:
+    """Every tensor lives on the current device."""
+    d = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.get_device() != d:
+            raise ValueError("fellm_amd ops need device tensors (no CPU fallback)" if t.get_device() < 0 else
+                             "tensors are not on the current device")
 
 
-def _u32(name: str, t: torch.Tensor | None, numel: int | None = None) -> None:
-    """An int32 tensor (read as u32) of numel elements."""
-    if t is None:
-        return
+def _rows(t: torch.Tensor, rows: int, width: int) -> int:
+    """Row stride of a matrix ``[rows, width]`` with dense rows, such as a
+    column slice of a projection's output."""
+    if t.shape != (rows, width):
+        raise ValueError(f"expected a [{rows}, {width}] tensor, got {list(t.shape)}")
+    if t.is_contiguous() or rows <= 1 and (width <= 1 or t.stride(1) == 1):
+        return width
+    stride, step = t.stride()
+    if (step != 1 and width > 1) or stride < width:
+        raise ValueError("rows must be dense and must not overlap")
+    return stride
+
+
+def _u32(name: str, t: torch.Tensor, numel: int) -> None:
+    """A dense int32 tensor (read as u32) of numel elements."""
     if t.dtype != torch.int32:
         raise TypeError(f"{name} must be int32")
-    if numel is not None and t.numel() != numel:
-        raise ValueError(f"{name} must have {numel} elements, not {t.numel()}")
-
-
-def _same_device(first: torch.Tensor, *ts: torch.Tensor | None) -> None:
-    for t in ts:
-        if t is not None and t.device != first.device:
-            raise ValueError("tensors are on different devices")
-    if first.device.index != torch.cuda.current_device():
-        raise ValueError("tensors are not on the current device")
+    if t.numel() != numel or not t.is_contiguous():
+        raise ValueError(f"{name} must be dense and have {numel} elements, not {t.numel()}")
 
 
 def _p(t: torch.Tensor | None) -> int | None:
@@ -222,19 +218,9 @@ class PagedKvCache:
         return (2 * block_size * stride * 2 + 63) // 64 * 64
 
     def c_struct(self, layer: int) -> _lib.FellmRocmPagedKv:
-        s = _lib.FellmRocmPagedKv()
-        s.arena = self.arena.data_ptr()
-        s.arena_len = self.arena.numel()
-        s.block_table = self.block_table.data_ptr()
-        s.n_block_table = self.block_table.numel()
-        s.n_logical_blocks = self.n_logical_blocks
-        s.n_layers = self.n_layers
-        s.layer = layer
-        s.block_size = self.block_size
-        s.block_bytes = self.block_bytes
-        s.stride = self.stride
-        s.kv_dtype = int(_ACT[self.kv_dtype])
-        return s
+        return _lib.FellmRocmPagedKv(self.arena.data_ptr(), self.arena.numel(), self.block_table.data_ptr(),
+                                     self.block_table.numel(), self.n_logical_blocks, self.n_layers, layer,
+                                     self.block_size, self.block_bytes, self.stride, _ACT_CODE[self.kv_dtype])
 
 
 def kv_write(rows, kv_positions, cache: PagedKvCache, *, layer: int = 0, is_v: bool = False, err_flag=None):
@@ -263,33 +249,36 @@ def rope_kv_write(q, k, v, inv_freqs, kv_positions, cache: PagedKvCache, *, head
 
 
 def _norm_args(q, k, q_weight, k_weight, inv_freqs, head_dim, rope_dim):
-    """Checks shared by the per-head norm ops: (q stride, k stride, q heads, KV heads)."""
-    if head_dim <= 0 or q.shape[-1] % head_dim or k.shape[-1] % head_dim:
+    """Checks shared by the per-head norm ops: (rows, q stride, k stride, q heads, KV heads)."""
+    if q.dim() != 2 or k.dim() != 2:
+        raise ValueError("q and k must be [rows, heads * head_dim]")
+    rows, qw = q.shape
+    kw = k.shape[1]
+    if head_dim <= 0 or qw % head_dim or kw % head_dim:
         raise ValueError("q and k rows must be whole heads of head_dim")
-    qs, ks = _rows(q), _rows(k)
-    if q.shape[0] != k.shape[0] or q.dtype != k.dtype:
-        raise ValueError("q and k must have the same rows and dtype")
-    _dev(q_weight, k_weight, inv_freqs)
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+    if q.dtype != k.dtype:
+        raise ValueError("q and k must have the same dtype")
+    qs, ks = _rows(q, rows, qw), _rows(k, rows, kw)
+    for w in (q_weight, k_weight):
         if w.dtype != torch.float32:
-            raise TypeError(f"{name} must be float32")
-        if w.numel() != head_dim:
-            raise ValueError(f"{name} must have head_dim elements")
+            raise TypeError("the norm weights must be float32")
+        if w.numel() != head_dim or not w.is_contiguous():
+            raise ValueError("the norm weights must be dense and have head_dim elements")
     if rope_dim:
         if inv_freqs.dtype != torch.float32:
             raise TypeError("inv_freqs must be float32")
-        if inv_freqs.numel() < rope_dim // 2:
-            raise ValueError("inv_freqs must have rope_dim / 2 elements")
-    return qs, ks, q.shape[1] // head_dim, k.shape[1] // head_dim
+        if inv_freqs.numel() < rope_dim // 2 or not inv_freqs.is_contiguous():
+            raise ValueError("inv_freqs must be dense and have rope_dim / 2 elements")
+    return rows, qs, ks, qw // head_dim, kw // head_dim
 
 
-def _rows_out(out, like):
-    """The output given for rows like `like`, checked, or a new dense one."""
+def _rows_out(out, like, rows, width):
+    """The output for rows like `like` and its row stride: the one given, checked, or a new dense one."""
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
-    if out.shape != like.shape or out.dtype != like.dtype:
-        raise ValueError("an output must have its input's shape and dtype")
-    return out
+        return torch.empty_like(like, memory_format=torch.contiguous_format), width
+    if out.dtype != like.dtype:
+        raise ValueError("an output must have its input's dtype")
+    return out, _rows(out, rows, width)
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, eps: float, inv_freqs, *, head_dim: int, rope_dim: int | None = None,
@@ -301,15 +290,15 @@ def qk_norm_rope(q, k, q_weight, k_weight, eps: float, inv_freqs, *, head_dim: i
     ``[head_dim]``; the rotation takes `rope`'s arguments.  Returns (q_out, k_out).
     """
     rope_dim = head_dim if rope_dim is None else rope_dim
-    qs, ks, nq, nk = _norm_args(q, k, q_weight, k_weight, inv_freqs, head_dim, rope_dim)
-    _dev(positions)
-    _u32("positions", positions, q.shape[0])
-    q_out = q if inplace else _rows_out(q_out, q)
-    k_out = k if inplace else _rows_out(k_out, k)
-    _same_device(q, k, q_weight, k_weight, inv_freqs, positions, q_out, k_out)
-    _lib.call("fellm_rocm_qk_norm_rope", _p(q), qs, _p(q_out), _rows(q_out), nq, _p(k), ks, _p(k_out), _rows(k_out), nk,
-              _code(q), q.shape[0], head_dim, rope_dim, pairing, _p(q_weight), _p(k_weight), eps, _p(inv_freqs),
-              _p(positions), position0, _stream())
+    rows, qs, ks, nq, nk = _norm_args(q, k, q_weight, k_weight, inv_freqs, head_dim, rope_dim)
+    if positions is not None:
+        _u32("positions", positions, rows)
+    q_out, qos = (q, qs) if inplace else _rows_out(q_out, q, rows, nq * head_dim)
+    k_out, kos = (k, ks) if inplace else _rows_out(k_out, k, rows, nk * head_dim)
+    _here(q, k, q_weight, k_weight, inv_freqs, positions, q_out, k_out)
+    _lib.call("fellm_rocm_qk_norm_rope", _p(q), qs, _p(q_out), qos, nq, _p(k), ks, _p(k_out), kos, nk, _code(q), rows,
+              head_dim, rope_dim, pairing, _p(q_weight), _p(k_weight), eps, _p(inv_freqs), _p(positions), position0,
+              _stream())
     return q_out, k_out
 
 
@@ -323,23 +312,26 @@ def qk_norm_rope_kv_write(q, k, v, q_weight, k_weight, eps: float, inv_freqs, kv
     (default: r).  ``k_out``, if given, gets the rotated K rows.  Returns q_out.
     """
     rope_dim = head_dim if rope_dim is None else rope_dim
-    qs, ks, nq, nk = _norm_args(q, k, q_weight, k_weight, inv_freqs, head_dim, rope_dim)
-    rows = q.shape[0]
-    vs = _rows(v, k.shape[1])
-    if v.shape[0] != rows or v.dtype != q.dtype:
-        raise ValueError("v must have k's rows and dtype")
-    _dev(kv_positions, rope_positions, sequences, k_out, err_flag)
-    for name, t in (("kv_positions", kv_positions), ("rope_positions", rope_positions), ("sequences", sequences)):
-        _u32(name, t, rows)
-    _u32("err_flag", err_flag)
-    q_out = q if inplace_q else _rows_out(q_out, q)
-    if k_out is not None:
-        _rows_out(k_out, k)
-    _same_device(q, k, v, q_weight, k_weight, inv_freqs, kv_positions, rope_positions, sequences, q_out, k_out,
-                 cache.arena, cache.block_table, err_flag)
+    rows, qs, ks, nq, nk = _norm_args(q, k, q_weight, k_weight, inv_freqs, head_dim, rope_dim)
+    kw = nk * head_dim
+    vs = _rows(v, rows, kw)
+    if v.dtype != q.dtype:
+        raise ValueError("v must have k's dtype")
+    _u32("kv_positions", kv_positions, rows)
+    if rope_positions is not None:
+        _u32("rope_positions", rope_positions, rows)
+    if sequences is not None:
+        _u32("sequences", sequences, rows)
+    if err_flag is not None:
+        _u32("err_flag", err_flag, 1)
+    q_out, qos = (q, qs) if inplace_q else _rows_out(q_out, q, rows, nq * head_dim)
+    if k_out is not None and _rows_out(k_out, k, rows, kw)[1] != kw:
+        raise ValueError("k_out must be dense")
+    _here(q, k, v, q_weight, k_weight, inv_freqs, kv_positions, rope_positions, sequences, q_out, k_out, cache.arena,
+          cache.block_table, err_flag)
     kv = cache.c_struct(layer)
-    _lib.call("fellm_rocm_qk_norm_rope_kv_write", _p(q), qs, _p(q_out), _rows(q_out), nq, _p(k), ks, _p(k_out), _p(v), vs,
-              nk, _code(q), rows, head_dim, rope_dim, pairing, _p(q_weight), _p(k_weight), eps, _p(inv_freqs),
+    _lib.call("fellm_rocm_qk_norm_rope_kv_write", _p(q), qs, _p(q_out), qos, nq, _p(k), ks, _p(k_out), _p(v), vs, nk,
+              _code(q), rows, head_dim, rope_dim, pairing, _p(q_weight), _p(k_weight), eps, _p(inv_freqs),
               _p(rope_positions), _p(kv_positions), _p(sequences), C.byref(kv), _p(err_flag), _stream())
     return q_out
 
@@ -397,21 +389,21 @@ def prompt_attention(q, k, v, cu_seqlens, *, n_heads: int, n_kv_heads: int, head
     allowed), ``cu_seqlens`` int32 device ``[sequences + 1]`` with the first
     token of each sequence.  Returns out ``[tokens, n_heads*head_dim]``, in which
     rows of no sequence are left as they were."""
-    qs = _rows(q, n_heads * head_dim)
-    ks, vs = (_rows(t, n_kv_heads * head_dim) for t in (k, v))
-    tokens = q.shape[0]
-    if any(t.shape[0] != tokens or t.dtype != q.dtype for t in (k, v)):
-        raise ValueError("q, k and v must have the same rows and dtype")
-    _dev(cu_seqlens, out)
-    _u32("cu_seqlens", cu_seqlens)
-    if cu_seqlens.numel() < 1:
+    tokens, qw, kw = q.shape[0], n_heads * head_dim, n_kv_heads * head_dim
+    qs, ks, vs = _rows(q, tokens, qw), _rows(k, tokens, kw), _rows(v, tokens, kw)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must have the same dtype")
+    n_seqs = cu_seqlens.numel() - 1
+    if n_seqs < 0:
         raise ValueError("cu_seqlens must have sequences + 1 elements")
-    out = out if out is not None else torch.empty((tokens, n_heads * head_dim), dtype=q.dtype, device=q.device)
-    if out.numel() != tokens * n_heads * head_dim or out.dtype != q.dtype:
-        raise ValueError("out must have q's shape and dtype")
-    _same_device(q, k, v, cu_seqlens, out)
-    _lib.call("fellm_rocm_prompt_attention", _p(q), qs, _p(k), ks, _p(v), vs, _p(out), _code(q), _p(cu_seqlens),
-              cu_seqlens.numel() - 1, tokens, n_heads, n_kv_heads, head_dim, scale, int(causal), window, _stream())
+    _u32("cu_seqlens", cu_seqlens, n_seqs + 1)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.numel() != tokens * qw or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("out must be dense and have q's shape and dtype")
+    _here(q, k, v, cu_seqlens, out)
+    _lib.call("fellm_rocm_prompt_attention", _p(q), qs, _p(k), ks, _p(v), vs, _p(out), _code(q), _p(cu_seqlens), n_seqs,
+              tokens, n_heads, n_kv_heads, head_dim, scale, int(causal), window, _stream())
     return out
 
 
@@ -428,31 +420,33 @@ def paged_tree_attention(q, cu_nodes, prefix_lengths, cache: PagedKvCache, *, n_
     sequence's new token j; None: causal (a chunk of a prompt), with an optional
     ``window``.  ``max_nodes`` and ``max_prefix`` bound the counts.  Returns out
     in out_dtype (default: q's dtype)."""
-    _dev(q, cu_nodes, prefix_lengths, tree_mask, out, workspace)
-    tokens = q.shape[0]
-    if q.numel() != tokens * n_heads * head_dim:
-        raise ValueError("q rows must be n_heads heads of head_dim")
-    _u32("cu_nodes", cu_nodes)
+    tokens, qw = q.shape[0], n_heads * head_dim
+    if _rows(q, tokens, qw) != qw:
+        raise ValueError("q must be dense")
     n_seqs = cu_nodes.numel() - 1
     if n_seqs < 0:
         raise ValueError("cu_nodes must have sequences + 1 elements")
+    _u32("cu_nodes", cu_nodes, n_seqs + 1)
     _u32("prefix_lengths", prefix_lengths, n_seqs)
     words = 0
     if tree_mask is not None:
-        _u32("tree_mask", tree_mask)
         if tree_mask.dim() != 2 or tree_mask.shape[0] != tokens:
             raise ValueError("tree_mask must be [tokens, words]")
         words = tree_mask.shape[1]
-    out_dtype = out_dtype or (q.dtype if out is None else out.dtype)
-    out = out if out is not None else torch.empty((tokens, n_heads * head_dim), dtype=out_dtype, device=q.device)
-    if out.numel() != q.numel() or out.dtype != out_dtype:
-        raise ValueError("out must have q's shape and the output dtype")
-    need = _lib.lib().fellm_rocm_paged_tree_attention_workspace(n_seqs, tokens, n_heads, n_kv_heads, head_dim, max_nodes,
-                                                                max_prefix)
-    if workspace is None and need:
-        workspace = torch.empty(need // 4, dtype=torch.float32, device=q.device)
+        _u32("tree_mask", tree_mask, tokens * words)
+    if out is None:
+        out = torch.empty((tokens, qw), dtype=out_dtype or q.dtype, device=q.device)
+    elif out.numel() != tokens * qw or not out.is_contiguous() or (out_dtype and out.dtype != out_dtype):
+        raise ValueError("out must be dense and have q's shape and the output dtype")
+    if workspace is None:
+        need = _lib.lib().fellm_rocm_paged_tree_attention_workspace(n_seqs, tokens, n_heads, n_kv_heads, head_dim,
+                                                                    max_nodes, max_prefix)
+        if need:
+            workspace = torch.empty(need // 4, dtype=torch.float32, device=q.device)
+    elif not workspace.is_contiguous():
+        raise ValueError("workspace must be dense")
     ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
-    _same_device(q, cu_nodes, prefix_lengths, tree_mask, out, workspace, cache.arena, cache.block_table)
+    _here(q, cu_nodes, prefix_lengths, tree_mask, out, workspace, cache.arena, cache.block_table)
     kv = cache.c_struct(layer)
     _lib.call("fellm_rocm_paged_tree_attention", _p(q), _code(q), _p(out), _code(out), _p(cu_nodes), _p(prefix_lengths),
               n_seqs, tokens, _p(tree_mask), words, n_heads, n_kv_heads, head_dim, max_nodes, max_prefix, scale, window,
