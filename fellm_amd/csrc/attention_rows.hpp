@@ -303,20 +303,18 @@ __device__ __forceinline__ const uint8_t *key_ptr(const Args &a, const Tile &t, 
     }
 }
 
-__device__ __forceinline__ float load_elem(const void *p, uint32_t dtype, size_t i) {
-    if (dtype == FELLM_DTYPE_F32) return static_cast<const float *>(p)[i];
-    if (dtype == FELLM_DTYPE_F16) return F16::load(static_cast<const _Float16 *>(p)[i]);
-    return BF16::load(static_cast<const uint16_t *>(p)[i]);
-}
 __device__ __forceinline__ void store_elem(void *p, uint32_t dtype, size_t i, float v) {
     if (dtype == FELLM_DTYPE_F32) static_cast<float *>(p)[i] = v;
     else if (dtype == FELLM_DTYPE_F16) static_cast<_Float16 *>(p)[i] = F16::store(v);
     else static_cast<uint16_t *>(p)[i] = BF16::store(v);
 }
 
-// One row over the keys [k0, k1), by one wavefront, key by key: only attended
-// keys are touched.  Unnormalised sums in acc (dims lane + 64 e), m, l, all
-// times 2^bias as the tiles' are.
+// One row over the keys [k0, k1), by one wavefront: only attended keys count,
+// whatever the others hold.  A lane scores a key, then owns dims lane + 64 e.
+// Unnormalised sums in acc, m, l, all times 2^bias as the tiles' are; the row has
+// an attended key here.  The loads
+// of several keys are on their way together: a batch whose values all are NaN
+// takes this path everywhere.
 template <typename E, int HD, bool PAGED>
 __device__ void careful_row(const Args &a, const Tile &t, uint32_t g, uint32_t token, uint32_t head, uint32_t k0,
                             uint32_t k1, float bias, float (&acc)[HD / 64], float &m, float &l) {
@@ -327,8 +325,21 @@ __device__ void careful_row(const Args &a, const Tile &t, uint32_t g, uint32_t t
     auto score = [&](uint32_t j) -> float {
         const T *kp = reinterpret_cast<const T *>(key_ptr<PAGED>(a, t, g, HD, j, false));
         float s = 0.0f;
-#pragma unroll 1
-        for (int d = 0; d < HD; ++d) s = fmaf(load_elem(a.q, a.q_dtype, q0 + d), kp ? E::A::load(kp[d]) : 0.0f, s);
+#pragma unroll 4
+        for (int d = 0; d < HD; d += 8) {
+            float k8[8], q8[8];
+            if (kp) {
+                load_f32<typename E::A, 8>(kp + d, k8);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) k8[e] = 0.0f;
+            }
+            if (a.q_dtype == FELLM_DTYPE_F32) load_f32<F32, 8>(static_cast<const float *>(a.q) + q0 + d, q8);
+            else if (a.q_dtype == FELLM_DTYPE_F16) load_f32<F16, 8>(static_cast<const _Float16 *>(a.q) + q0 + d, q8);
+            else load_f32<BF16, 8>(static_cast<const uint16_t *>(a.q) + q0 + d, q8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = fmaf(q8[e], k8[e], s);
+        }
         return s;
     };
     auto attended = [&](uint32_t kb) -> uint64_t {
@@ -339,6 +350,7 @@ __device__ void careful_row(const Args &a, const Tile &t, uint32_t g, uint32_t t
     l = 0.0f;
 #pragma unroll
     for (int e = 0; e < HD / 64; ++e) acc[e] = 0.0f;
+#pragma unroll 1
     for (uint32_t kb = k0; kb < k1; kb += 64) {
         const uint64_t bits = attended(kb);
         if (bits >> lane & 1) {
@@ -347,22 +359,34 @@ __device__ void careful_row(const Args &a, const Tile &t, uint32_t g, uint32_t t
         }
     }
     float top = m;
-    bool nan = m != m;
+    const bool nan = m != m;
 #pragma unroll
     for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-    m = __any(nan) ? __builtin_nanf("") : top;
+    // scores that all are -inf: the lowest finite maximum keeps p = 0 and l = 0, so
+    // that the row is 0 / 0 alone and nothing next to other shares of its keys
+    m = __any(nan) ? __builtin_nanf("") : fmaxf(top, -3.402823466e38f);
+#pragma unroll 1
     for (uint32_t kb = k0; kb < k1; kb += 64) {
-        uint64_t bits = attended(kb);
+        const uint64_t bits = attended(kb);
         if (!bits) continue;
         const float p = bits >> lane & 1 ? __builtin_amdgcn_exp2f((score(kb + lane) - m) * a.c + bias) : 0.0f;
         l += p;
-        while (bits) {
-            const uint32_t b = (uint32_t)__builtin_ctzll(bits);
-            bits &= bits - 1;
-            const float pb = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), b));
-            const T *vp = reinterpret_cast<const T *>(key_ptr<PAGED>(a, t, g, HD, kb + b, true));
+#pragma unroll 1
+        for (uint32_t b0 = 0; b0 < 64 && kb + b0 < k1; b0 += 8) {
+            float v[8][HD / 64];
 #pragma unroll
-            for (int e = 0; e < HD / 64; ++e) acc[e] = fmaf(pb, vp ? E::A::load(vp[lane + 64 * e]) : 0.0f, acc[e]);
+            for (uint32_t b = 0; b < 8; ++b) {
+                const T *vp = reinterpret_cast<const T *>(key_ptr<PAGED>(a, t, g, HD, min(kb + b0 + b, k1 - 1), true));
+#pragma unroll
+                for (int e = 0; e < HD / 64; ++e) v[b][e] = vp ? E::A::load(vp[lane + 64 * e]) : 0.0f;
+            }
+#pragma unroll
+            for (uint32_t b = 0; b < 8; ++b) {
+                if (!(bits >> (b0 + b) & 1)) continue;
+                const float pb = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), b0 + b));
+#pragma unroll
+                for (int e = 0; e < HD / 64; ++e) acc[e] = fmaf(pb, v[b][e], acc[e]);
+            }
         }
     }
     l = wave_sum(l);
@@ -548,9 +572,9 @@ __device__ __forceinline__ Rsrc uniform_rsrc(const uint8_t *p, uint32_t range) {
 // wavefronts that share those rows and take every KW-th key tile, KT: keys of
 // a wavefront's tile (32 or 64), PARTS: q and p held to f32 accuracy in several
 // 16-bit parts (q or out in f32, or q of another 16-bit type than K/V).
-// OCC: wavefronts per SIMD the registers are kept for.  NST: key tiles in LDS
-// (NST - 1 on their way while one is worked on).
-template <typename E, int HD, int RW, int KW, int KT, bool PAGED, bool PARTS, int OCC, int NST = 2>
+// OCC: wavefronts per SIMD the registers are kept for.  (Three tiles in LDS
+// instead of two, two of them on their way, measured the same within 1%.)
+template <typename E, int HD, int RW, int KW, int KT, bool PAGED, bool PARTS, int OCC>
 __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     constexpr int NW = RW * KW, NS = HD / 16, NU = KT / 32, ND = HD / 32;
     constexpr int QP = PARTS ? E::kQParts : 1, PP = PARTS ? E::kPParts : 1;
@@ -565,7 +589,6 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     // Separate arrays: the compiler then knows that a read of one need not wait
     // for loads to another.
     __shared__ __align__(16) uint8_t k_lds0[TK * RB], v_lds0[TK * RB], k_lds1[TK * RB], v_lds1[TK * RB];
-    __shared__ __align__(16) uint8_t k_lds2[NST > 2 ? TK * RB : 16], v_lds2[NST > 2 ? TK * RB : 16];
 
     const uint32_t lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const uint32_t rw = wave % RW, kw = wave / RW;
@@ -584,364 +607,352 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
         x_end = min(line.units, x + line.share);
     }
     for (uint32_t again = 0; x < x_end; again = 1) {
-    Tile t;
-    Keys sh;
-    bool direct = true;
-    float *part = nullptr;  // the tile's records where others share it
-    if constexpr (PAGED) {
-        const auto spot = line.template find<false>(x);
-        t = spot.t;
-        if (t.n == 0) break;  // offsets that are none: nothing more to find
-        sh = tile_keys<BM>(a, t);
-        const uint32_t u0 = x - spot.at, u1 = min(spot.units, u0 + x_end - x);
-        direct = u1 - u0 == spot.units;
-        if (!direct) {
-            part = a.part + (size_t)(2 * (g * ids + id) + again) * BM * kRec<HD>;
-            const uint32_t lo = sh.begin;
-            sh.begin = lo + u0 * line.per * TK;
-            if (u1 < spot.units) sh.end = min(sh.end, lo + u1 * line.per * TK);
-        }
-        x += u1 - u0;
-        if (again) __syncthreads();  // the buffers may still be read for the tile before
-    } else {
-        t = tile_of<BM>(a, id, ids);
-        if (t.n == 0) return;
-        sh = tile_keys<BM>(a, t);
-        ++x;
-    }
-
-    const uint32_t row = t.row0 + rw * kRows + n;
-    const bool valid = row < t.n * a.group;
-    const uint32_t rrow = valid ? row : t.n * a.group - 1;
-    const uint32_t token = a.by_group(rrow), head = g * a.group + rrow - token * a.group;
-    const KeyRange mine = row_keys(a, t, token);
-    // keys that every row of this wavefront attends, and that any does
-    const uint32_t w0 = min(t.row0 + rw * kRows, t.n * a.group - 1), w1 = min(w0 + kRows - 1, t.n * a.group - 1);
-    const KeyRange rf = row_keys(a, t, a.by_group(w0)), rl = row_keys(a, t, a.by_group(w1));
-    const uint32_t full_lo = rl.lo, full_hi = a.mask ? t.before : rf.hi, any_lo = rf.lo, any_hi = rl.hi;
-
-    f32x16 acc[ND];
-    float m = -__builtin_inff(), l = 0.0f;
-    bool some = false;  // the row attends a key of this share
-#pragma unroll
-    for (int d = 0; d < ND; ++d) acc[d] = f32x16(0.0f);
-
-    // ---- staging: SK keys from kb + wave SK on
-    const uint32_t skey = lane / CH, spos = lane % CH;
-    constexpr uint32_t BK = SK < kBlockTokens ? SK : kBlockTokens;  // keys of a piece, of one cache block
-    // Table entries of the pieces of the tile that is requested next (paged): read
-    // a tile ahead, so that their latency does not stand before the request.
-    uint32_t entry[SK / BK];
-    auto look_up = [&](uint32_t kb) __attribute__((always_inline)) {
+        Tile t;
+        Keys sh;
+        bool direct = true;
+        float *part = nullptr;  // the tile's records where others share it
         if constexpr (PAGED) {
-#pragma unroll
-            for (uint32_t b = 0; b < SK / BK; ++b) {
-                // through a vector load: a scalar one on its way would turn every
-                // wait for an LDS read into a wait for all of them
-                uint32_t blk = (kb + wave * SK + b * BK) / kBlockTokens;
-                __asm__("" : "+v"(blk));
-                entry[b] = block_entry(a, t, blk);
+            const auto spot = line.template find<false>(x);
+            t = spot.t;
+            if (t.n == 0) break;  // offsets that are none: nothing more to find
+            sh = tile_keys<BM>(a, t);
+            const uint32_t u0 = x - spot.at, u1 = min(spot.units, u0 + x_end - x);
+            direct = u1 - u0 == spot.units;
+            if (!direct) {
+                part = a.part + (size_t)(2 * (g * ids + id) + again) * BM * kRec<HD>;
+                const uint32_t lo = sh.begin;
+                sh.begin = lo + u0 * line.per * TK;
+                if (u1 < spot.units) sh.end = min(sh.end, lo + u1 * line.per * TK);
             }
+            x += u1 - u0;
+            if (again) __syncthreads();  // the buffers may still be read for the tile before
+        } else {
+            t = tile_of<BM>(a, id, ids);
+            if (t.n == 0) return;
+            sh = tile_keys<BM>(a, t);
+            ++x;
         }
-    };
-    auto stage = [&](uint32_t kb, uint8_t *lds, bool is_v) __attribute__((always_inline)) {
-#pragma unroll
-        for (uint32_t b0 = 0; b0 < SK; b0 += BK) {
-            const uint32_t j = kb + wave * SK + b0;
-            const uint32_t have = j < sh.end ? min(BK, sh.end - j) : 0;
-            const uint32_t stride = (PAGED ? a.stride : is_v ? a.v_stride : a.k_stride) * 2;
-            const uint8_t *src;
+
+        const uint32_t row = t.row0 + rw * kRows + n;
+        const bool valid = row < t.n * a.group;
+        const uint32_t rrow = valid ? row : t.n * a.group - 1;
+        const uint32_t token = a.by_group(rrow), head = g * a.group + rrow - token * a.group;
+        const KeyRange mine = row_keys(a, t, token);
+        // keys that every row of this wavefront attends, and that any does
+        const uint32_t w0 = min(t.row0 + rw * kRows, t.n * a.group - 1), w1 = min(w0 + kRows - 1, t.n * a.group - 1);
+        const KeyRange rf = row_keys(a, t, a.by_group(w0)), rl = row_keys(a, t, a.by_group(w1));
+        const uint32_t full_lo = rl.lo, full_hi = a.mask ? t.before : rf.hi, any_lo = rf.lo, any_hi = rl.hi;
+
+        f32x16 acc[ND];
+        float m = -__builtin_inff(), l = 0.0f;
+        bool some = false;  // the row attends a key of this share
+    #pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] = f32x16(0.0f);
+
+        // ---- staging: SK keys from kb + wave SK on
+        const uint32_t skey = lane / CH, spos = lane % CH;
+        constexpr uint32_t BK = SK < kBlockTokens ? SK : kBlockTokens;  // keys of a piece, of one cache block
+        // Table entries of the pieces of the tile that is requested next (paged): read
+        // a tile ahead, so that their latency does not stand before the request.
+        uint32_t entry[SK / BK];
+        auto look_up = [&](uint32_t kb) __attribute__((always_inline)) {
             if constexpr (PAGED) {
-                const uint8_t *at = block_ptr(a, __builtin_amdgcn_readfirstlane(entry[b0 / BK]));
-                src = at ? at + (j % kBlockTokens + (is_v ? kBlockTokens : 0)) * stride + g * RB : nullptr;
-            } else {
-                src = key_ptr<PAGED>(a, t, g, HD, j, is_v);
+    #pragma unroll
+                for (uint32_t b = 0; b < SK / BK; ++b) {
+                    // through a vector load: a scalar one on its way would turn every
+                    // wait for an LDS read into a wait for all of them
+                    uint32_t blk = (kb + wave * SK + b * BK) / kBlockTokens;
+                    __asm__("" : "+v"(blk));
+                    entry[b] = block_entry(a, t, blk);
+                }
             }
-            const Rsrc rs = uniform_rsrc(src, src && have ? (have - 1) * stride + RB : 0);
-#pragma unroll
-            for (uint32_t i = 0; i < BK / KPI; ++i) {
-                const uint32_t key = i * KPI + skey;  // inside the piece of BK keys
-                const uint32_t c = (spos ^ swizzle<HD>(wave * SK + b0 + key)) * 16;
-                using L = __attribute__((address_space(3))) void;
-                const uint32_t at = (wave * SK + b0 + i * KPI) * RB;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (L *)(lds + at), 16, key * stride + c, 0, 0, 0);
-            }
-        }
-    };
-    auto request = [&](uint32_t kb, uint8_t *kl, uint8_t *vl) __attribute__((always_inline)) {
-        if (kb >= sh.end) return;
-        stage(kb, kl, false);
-        stage(kb, vl, true);
-        look_up(kb + TK);
-    };
-
-    look_up(sh.begin);
-    request(sh.begin, k_lds0, v_lds0);
-    if constexpr (NST > 2) request(sh.begin + TK, k_lds1, v_lds1);
-
-    // Q^T as the B operand: row n, dims 16 st + 8 h .. +7
-    u32x4 qf[NS][QP];
-    {
-        const size_t q0 = (size_t)(t.first + token) * a.q_stride + (size_t)head * HD + 8 * h;
-        if constexpr (!PARTS) {
-            const T *qp = static_cast<const T *>(a.q) + q0;
-#pragma unroll
-            for (int s = 0; s < NS; ++s) qf[s][0] = *reinterpret_cast<const u32x4 *>(qp + 16 * s);
-        } else {
-#pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                float x[8];
-                if (a.q_dtype == FELLM_DTYPE_F32) load_f32<F32, 8>(static_cast<const float *>(a.q) + q0 + 16 * s, x);
-                else if (a.q_dtype == FELLM_DTYPE_F16) load_f32<F16, 8>(static_cast<const _Float16 *>(a.q) + q0 + 16 * s, x);
-                else load_f32<BF16, 8>(static_cast<const uint16_t *>(a.q) + q0 + 16 * s, x);
-#pragma unroll
-                for (int p = 0; p < QP; ++p)
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) qf[s][p][w] = E::part(x[2 * w], x[2 * w + 1]);
-            }
-        }
-    }
-
-    // ---- a tile of KT keys from kb on, in three parts
-    f32x16 s[NU];          // scores of row n
-    u32x4 pf[KT / 16][PP]; // probabilities, as the second product takes them
-    const uint32_t kbase = kw * KT * RB + n * RB, ksw = (h ^ swizzle<HD>(n)) * 16;
-    auto scores = [&](const uint8_t *kl) __attribute__((always_inline)) {
-        // Piece x: dims 16 (x / NU) .. of keys 32 (x % NU) ...  Each is read kAhead
-        // products early and the order is fixed: left to itself the compiler reads
-        // a piece right before its product and waits for the LDS every time (one
-        // prompt of 16384 tokens, 32/4 heads of 128, bf16: 2114 -> 1939 us).
-        constexpr int N = NS * NU, kAhead = 4;
-        auto piece = [&](int x) {
-            return *reinterpret_cast<const u32x4 *>(kl + kbase + x % NU * 32 * RB + (ksw ^ (x / NU * 32)));
         };
-        u32x4 kf[kAhead];
-#pragma unroll
-        for (int x = 0; x < kAhead; ++x) kf[x] = piece(x);
-#pragma unroll
-        for (int u = 0; u < NU; ++u) s[u] = f32x16(0.0f);
-#pragma unroll
-        for (int x = 0; x < N; ++x) {
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int p = 0; p < QP; ++p) s[x % NU] = E::mfma(kf[x % kAhead], qf[x / NU][p], s[x % NU]);
-            if (x + kAhead < N) kf[x % kAhead] = piece(x + kAhead);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    auto weights = [&](uint32_t kb) __attribute__((always_inline)) {
-        if (!(kb >= full_lo && kb + KT <= full_hi && kb + KT <= sh.end)) {
-            uint64_t bits = key_bits(a, t, token, mine, kb);
-            if (kb + 64 > sh.end) bits &= (1ull << (sh.end - kb)) - 1;
-            some |= (KT == 64 ? bits : (uint32_t)bits) != 0;
-            bits >>= 4 * h;
-#pragma unroll
-            for (int u = 0; u < NU; ++u)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!(bits >> (32 * u + 8 * (i / 4) + i % 4) & 1)) s[u][i] = -__builtin_inff();
-        } else {
-            some = true;
-        }
-        float top = s[0][0];
-#pragma unroll
-        for (int u = 0; u < NU; ++u)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
-        top = halves_max(top);
-        if (__any((top - m) * a.c > kLazy)) {
-            const float mn = fmaxf(m, top);
-            const float f = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * a.c);
-            m = mn;
-            l *= f;
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[d][i] *= f;
-        }
-        const float base = (m == -__builtin_inff() ? 0.0f : -m * a.c) + kBias;
-        float sum = 0.0f;
-#pragma unroll
-        for (int k = 0; k < KT / 16; ++k) {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[e] = __builtin_amdgcn_exp2f(fmaf(s[k / 2][8 * (k % 2) + e], a.c, base));
-                sum += x[e];
+        auto stage = [&](uint32_t kb, uint8_t *lds, bool is_v) __attribute__((always_inline)) {
+    #pragma unroll
+            for (uint32_t b0 = 0; b0 < SK; b0 += BK) {
+                const uint32_t j = kb + wave * SK + b0;
+                const uint32_t have = j < sh.end ? min(BK, sh.end - j) : 0;
+                const uint32_t stride = (PAGED ? a.stride : is_v ? a.v_stride : a.k_stride) * 2;
+                const uint8_t *src;
+                if constexpr (PAGED) {
+                    const uint8_t *at = block_ptr(a, __builtin_amdgcn_readfirstlane(entry[b0 / BK]));
+                    src = at ? at + (j % kBlockTokens + (is_v ? kBlockTokens : 0)) * stride + g * RB : nullptr;
+                } else {
+                    src = key_ptr<PAGED>(a, t, g, HD, j, is_v);
+                }
+                const Rsrc rs = uniform_rsrc(src, src && have ? (have - 1) * stride + RB : 0);
+    #pragma unroll
+                for (uint32_t i = 0; i < BK / KPI; ++i) {
+                    const uint32_t key = i * KPI + skey;  // inside the piece of BK keys
+                    const uint32_t c = (spos ^ swizzle<HD>(wave * SK + b0 + key)) * 16;
+                    using L = __attribute__((address_space(3))) void;
+                    const uint32_t at = (wave * SK + b0 + i * KPI) * RB;
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (L *)(lds + at), 16, key * stride + c, 0, 0, 0);
+                }
             }
-#pragma unroll
-            for (int p = 0; p < PP; ++p)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) pf[k][p][w] = E::part(x[2 * w], x[2 * w + 1]);
-        }
-        l += sum;
-    };
-    // V^T pieces: lane group of 16 reads keys 4 h + .. of dims 16 (group % 2) ..
-    const uint32_t vkey = 4 * h + lane % 16 / 4, vpc = lane / 16 % 2 * 2 + lane % 4 / 2;
-    const uint32_t vbase = kw * KT * RB + vkey * RB + lane % 2 * 8;
-    const uint32_t vsw0 = (vpc ^ swizzle<HD>(vkey)) * 16, vsw1 = (vpc ^ swizzle<HD>(vkey + 8)) * 16;
-    auto products = [&](const uint8_t *vl) __attribute__((always_inline)) {
-        using L4 = __attribute__((address_space(3))) s16x4;
-#pragma unroll
-        for (int k = 0; k < KT / 16; ++k)
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const uint32_t off = k * 16 * RB + vbase;
-                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L4 *)(vl + off + (vsw0 ^ (d * 64))));
-                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L4 *)(vl + off + 8 * RB + (vsw1 ^ (d * 64))));
-                const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
-                const u32x4 vf = {lo2[0], lo2[1], hi2[0], hi2[1]};
-#pragma unroll
-                for (int p = 0; p < PP; ++p) acc[d] = E::mfma(vf, pf[k][p], acc[d]);
-            }
-    };
-    const uint32_t hi_here = t.row0 + rw * kRows < t.n * a.group ? min(sh.end, any_hi) : 0;  // 0: no row of its own
-    auto mine_at = [&](uint32_t kb) { return kb < hi_here && kb + KT > any_lo; };
+        };
+        auto request = [&](uint32_t kb, uint8_t *kl, uint8_t *vl) __attribute__((always_inline)) {
+            if (kb >= sh.end) return;
+            stage(kb, kl, false);
+            stage(kb, vl, true);
+            look_up(kb + TK);
+        };
 
-    // The oldest tile's loads to LDS are done, then everyone's.  The wait is
-    // written out: a barrier alone does not imply it, and the one the compiler
-    // puts before the reads cannot know of other wavefronts' loads.  Loads finish
-    // in order, so those of the NST - 2 tiles requested later may still be on
-    // their way (`newer`: there are such).
-    constexpr int kLater = (NST - 2) * 2 * (int)(SK / KPI);
-    static_assert(NST <= 3 && kLater < 16);
-    auto arrived = [&](bool newer) __attribute__((always_inline)) {
-        __asm__ volatile("" ::: "memory");
-        if (NST > 2 && newer) __builtin_amdgcn_s_waitcnt(0x0f70 | kLater);  // vmcnt(kLater)
-        else __builtin_amdgcn_s_waitcnt(0x0f70);                            // vmcnt(0)
-        __asm__ volatile("" ::: "memory");
-        __syncthreads();
-    };
-    // kn and vn: the buffers of the tile before, which no wavefront reads any more after the barrier
-    auto round = [&](uint32_t kb, const uint8_t *kl, const uint8_t *vl, uint8_t *kn, uint8_t *vn) __attribute__((always_inline)) {
-        if (kb >= sh.end) return;
-        arrived(kb + TK < sh.end);
-        request(kb + (NST - 1) * TK, kn, vn);
-        const uint32_t my = kb + kw * KT;
-        if (mine_at(my)) {
-            scores(kl);
-            weights(my);
-            products(vl);
+        look_up(sh.begin);
+        request(sh.begin, k_lds0, v_lds0);
+
+        // Q^T as the B operand: row n, dims 16 st + 8 h .. +7
+        u32x4 qf[NS][QP];
+        {
+            const size_t q0 = (size_t)(t.first + token) * a.q_stride + (size_t)head * HD + 8 * h;
+            if constexpr (!PARTS) {
+                const T *qp = static_cast<const T *>(a.q) + q0;
+    #pragma unroll
+                for (int s = 0; s < NS; ++s) qf[s][0] = *reinterpret_cast<const u32x4 *>(qp + 16 * s);
+            } else {
+    #pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    float x[8];
+                    if (a.q_dtype == FELLM_DTYPE_F32) load_f32<F32, 8>(static_cast<const float *>(a.q) + q0 + 16 * s, x);
+                    else if (a.q_dtype == FELLM_DTYPE_F16) load_f32<F16, 8>(static_cast<const _Float16 *>(a.q) + q0 + 16 * s, x);
+                    else load_f32<BF16, 8>(static_cast<const uint16_t *>(a.q) + q0 + 16 * s, x);
+    #pragma unroll
+                    for (int p = 0; p < QP; ++p)
+    #pragma unroll
+                        for (int w = 0; w < 4; ++w) qf[s][p][w] = E::part(x[2 * w], x[2 * w + 1]);
+                }
+            }
         }
-    };
-    for (uint32_t kb = sh.begin; kb < sh.end; kb += NST * TK) {
-        if constexpr (NST == 2) {
+
+        // ---- a tile of KT keys from kb on, in three parts
+        f32x16 s[NU];          // scores of row n
+        u32x4 pf[KT / 16][PP]; // probabilities, as the second product takes them
+        const uint32_t kbase = kw * KT * RB + n * RB, ksw = (h ^ swizzle<HD>(n)) * 16;
+        auto scores = [&](const uint8_t *kl) __attribute__((always_inline)) {
+            // Piece x: dims 16 (x / NU) .. of keys 32 (x % NU) ...  Each is read kAhead
+            // products early and the order is fixed: left to itself the compiler reads
+            // a piece right before its product and waits for the LDS every time (one
+            // prompt of 16384 tokens, 32/4 heads of 128, bf16: 2114 -> 1939 us).
+            constexpr int N = NS * NU, kAhead = 4;
+            auto piece = [&](int x) {
+                return *reinterpret_cast<const u32x4 *>(kl + kbase + x % NU * 32 * RB + (ksw ^ (x / NU * 32)));
+            };
+            u32x4 kf[kAhead];
+    #pragma unroll
+            for (int x = 0; x < kAhead; ++x) kf[x] = piece(x);
+    #pragma unroll
+            for (int u = 0; u < NU; ++u) s[u] = f32x16(0.0f);
+    #pragma unroll
+            for (int x = 0; x < N; ++x) {
+                __builtin_amdgcn_sched_barrier(0);
+    #pragma unroll
+                for (int p = 0; p < QP; ++p) s[x % NU] = E::mfma(kf[x % kAhead], qf[x / NU][p], s[x % NU]);
+                if (x + kAhead < N) kf[x % kAhead] = piece(x + kAhead);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto weights = [&](uint32_t kb) __attribute__((always_inline)) {
+            if (!(kb >= full_lo && kb + KT <= full_hi && kb + KT <= sh.end)) {
+                uint64_t bits = key_bits(a, t, token, mine, kb);
+                if (kb + 64 > sh.end) bits &= (1ull << (sh.end - kb)) - 1;
+                some |= (KT == 64 ? bits : (uint32_t)bits) != 0;
+                bits >>= 4 * h;
+    #pragma unroll
+                for (int u = 0; u < NU; ++u)
+    #pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (!(bits >> (32 * u + 8 * (i / 4) + i % 4) & 1)) s[u][i] = -__builtin_inff();
+            } else {
+                some = true;
+            }
+            float top = s[0][0];
+    #pragma unroll
+            for (int u = 0; u < NU; ++u)
+    #pragma unroll
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
+            top = halves_max(top);
+            if (__any((top - m) * a.c > kLazy)) {
+                const float mn = fmaxf(m, top);
+                const float f = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * a.c);
+                m = mn;
+                l *= f;
+    #pragma unroll
+                for (int d = 0; d < ND; ++d)
+    #pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+            }
+            const float base = (m == -__builtin_inff() ? 0.0f : -m * a.c) + kBias;
+            float sum = 0.0f;
+    #pragma unroll
+            for (int k = 0; k < KT / 16; ++k) {
+                float x[8];
+    #pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(fmaf(s[k / 2][8 * (k % 2) + e], a.c, base));
+                    sum += x[e];
+                }
+    #pragma unroll
+                for (int p = 0; p < PP; ++p)
+    #pragma unroll
+                    for (int w = 0; w < 4; ++w) pf[k][p][w] = E::part(x[2 * w], x[2 * w + 1]);
+            }
+            l += sum;
+        };
+        // V^T pieces: lane group of 16 reads keys 4 h + .. of dims 16 (group % 2) ..
+        const uint32_t vkey = 4 * h + lane % 16 / 4, vpc = lane / 16 % 2 * 2 + lane % 4 / 2;
+        const uint32_t vbase = kw * KT * RB + vkey * RB + lane % 2 * 8;
+        const uint32_t vsw0 = (vpc ^ swizzle<HD>(vkey)) * 16, vsw1 = (vpc ^ swizzle<HD>(vkey + 8)) * 16;
+        auto products = [&](const uint8_t *vl) __attribute__((always_inline)) {
+            using L4 = __attribute__((address_space(3))) s16x4;
+    #pragma unroll
+            for (int k = 0; k < KT / 16; ++k)
+    #pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    const uint32_t off = k * 16 * RB + vbase;
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L4 *)(vl + off + (vsw0 ^ (d * 64))));
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((L4 *)(vl + off + 8 * RB + (vsw1 ^ (d * 64))));
+                    const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
+                    const u32x4 vf = {lo2[0], lo2[1], hi2[0], hi2[1]};
+    #pragma unroll
+                    for (int p = 0; p < PP; ++p) acc[d] = E::mfma(vf, pf[k][p], acc[d]);
+                }
+        };
+        const uint32_t hi_here = t.row0 + rw * kRows < t.n * a.group ? min(sh.end, any_hi) : 0;  // 0: no row of its own
+        auto mine_at = [&](uint32_t kb) { return kb < hi_here && kb + KT > any_lo; };
+
+        // The tile's loads to LDS are done, then everyone's.  The wait is written out:
+        // a barrier alone does not imply it, and the one the compiler puts before the
+        // reads cannot know of other wavefronts' loads.
+        auto arrived = [&]() __attribute__((always_inline)) {
+            __asm__ volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+            __asm__ volatile("" ::: "memory");
+            __syncthreads();
+        };
+        // kn and vn: the buffers of the tile before, which no wavefront reads any more after the barrier
+        auto round = [&](uint32_t kb, const uint8_t *kl, const uint8_t *vl, uint8_t *kn, uint8_t *vn)
+                         __attribute__((always_inline)) {
+            if (kb >= sh.end) return;
+            arrived();
+            request(kb + TK, kn, vn);
+            const uint32_t my = kb + kw * KT;
+            if (mine_at(my)) {
+                scores(kl);
+                weights(my);
+                products(vl);
+            }
+        };
+        for (uint32_t kb = sh.begin; kb < sh.end; kb += 2 * TK) {
             round(kb, k_lds0, v_lds0, k_lds1, v_lds1);
             round(kb + TK, k_lds1, v_lds1, k_lds0, v_lds0);
-        } else {
-            round(kb, k_lds0, v_lds0, k_lds2, v_lds2);
-            round(kb + TK, k_lds1, v_lds1, k_lds0, v_lds0);
-            round(kb + 2 * TK, k_lds2, v_lds2, k_lds1, v_lds1);
         }
-    }
-    l = halves_sum(l);
+        l = halves_sum(l);
 
-    float probe = 0.0f;  // NaN if any sum is not finite
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) probe = fmaf(acc[d][i], 0.0f, probe);
-    probe = halves_sum(probe) + l * 0.0f;
-
-    // ---- wavefronts that share rows: every one leaves its sums in LDS and
-    // joins (and stores) the tiles d = kw, kw + KW, .. of all of them
-    if constexpr (KW > 1) {
-        static_assert(16 * RW <= KT, "the sums of all wavefronts fit the four buffers");
-        __shared__ float state_lds[NW][4][kWave];
-        auto sum_at = [&](uint32_t w, int x) -> float & {  // x-th of a lane's 16 ND sums
-            uint8_t *buf = x < 4 * ND ? k_lds0 : x < 8 * ND ? v_lds0 : x < 12 * ND ? k_lds1 : v_lds1;
-            return reinterpret_cast<float *>(buf)[(w * 4 * ND + x % (4 * ND)) * kWave + lane];
-        };
-        __syncthreads();
-#pragma unroll
+        float probe = 0.0f;  // NaN if any sum is not finite
+    #pragma unroll
         for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sum_at(wave, d * 16 + i) = acc[d][i];
-        state_lds[wave][0][lane] = m;
-        state_lds[wave][1][lane] = l;
-        state_lds[wave][2][lane] = probe;
-        state_lds[wave][3][lane] = some ? 1.0f : 0.0f;
-        __syncthreads();
-        float f[KW];
-        m = -__builtin_inff();
-#pragma unroll
-        for (int w = 0; w < KW; ++w) m = fmaxf(m, state_lds[rw + w * RW][0][lane]);
-        l = probe = 0.0f;
-#pragma unroll
-        for (int w = 0; w < KW; ++w) {
-            const float mw = state_lds[rw + w * RW][0][lane];
-            f[w] = mw == m ? 1.0f : __builtin_amdgcn_exp2f((mw - m) * a.c);
-            l = fmaf(state_lds[rw + w * RW][1][lane], f[w], l);
-            probe += state_lds[rw + w * RW][2][lane];
-            some |= state_lds[rw + w * RW][3][lane] != 0.0f;
-        }
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            if (d % KW != (int)kw) continue;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float v = 0.0f;
-#pragma unroll
-                for (int w = 0; w < KW; ++w) v = fmaf(sum_at(rw + w * RW, d * 16 + i), f[w], v);
-                acc[d][i] = v;
-            }
-        }
-    }
+    #pragma unroll
+            for (int i = 0; i < 16; ++i) probe = fmaf(acc[d][i], 0.0f, probe);
+        probe = halves_sum(probe) + l * 0.0f;
 
-    // ---- results
-    const bool bad = valid && some && !(probe == 0.0f && l > 0.0f);
-    // exchanges between a row's two lanes follow: both take part or neither, as
-    // valid and bad are the row's
-    if (valid && !bad) {
-        const float inv = !direct ? 1.0f : some ? 1.0f / l : 0.0f;
-        const size_t o0 = (size_t)(t.first + token) * a.out_stride + (size_t)head * HD;
-        float *rec = part + (size_t)(rw * kRows + n) * kRec<HD>;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            if (KW > 1 && d % KW != (int)kw) continue;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[d][i] *= inv;
-            if (!direct || (PARTS && a.out_dtype == FELLM_DTYPE_F32)) {
-                float *to = direct ? static_cast<float *>(a.out) + o0 : rec;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float v[4] = {acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
-                    store_f32<F32, 4>(to + 32 * d + 8 * i + 4 * h, v);
+        // ---- wavefronts that share rows: every one leaves its sums in LDS and
+        // joins (and stores) the tiles d = kw, kw + KW, .. of all of them
+        if constexpr (KW > 1) {
+            static_assert(16 * RW <= KT, "the sums of all wavefronts fit the four buffers");
+            __shared__ float state_lds[NW][4][kWave];
+            auto sum_at = [&](uint32_t w, int x) -> float & {  // x-th of a lane's 16 ND sums
+                uint8_t *buf = x < 4 * ND ? k_lds0 : x < 8 * ND ? v_lds0 : x < 12 * ND ? k_lds1 : v_lds1;
+                return reinterpret_cast<float *>(buf)[(w * 4 * ND + x % (4 * ND)) * kWave + lane];
+            };
+            __syncthreads();
+    #pragma unroll
+            for (int d = 0; d < ND; ++d)
+    #pragma unroll
+                for (int i = 0; i < 16; ++i) sum_at(wave, d * 16 + i) = acc[d][i];
+            state_lds[wave][0][lane] = m;
+            state_lds[wave][1][lane] = l;
+            state_lds[wave][2][lane] = probe;
+            state_lds[wave][3][lane] = some ? 1.0f : 0.0f;
+            __syncthreads();
+            float f[KW];
+            m = -__builtin_inff();
+    #pragma unroll
+            for (int w = 0; w < KW; ++w) m = fmaxf(m, state_lds[rw + w * RW][0][lane]);
+            l = probe = 0.0f;
+    #pragma unroll
+            for (int w = 0; w < KW; ++w) {
+                const float mw = state_lds[rw + w * RW][0][lane];
+                f[w] = mw == m ? 1.0f : __builtin_amdgcn_exp2f((mw - m) * a.c);
+                l = fmaf(state_lds[rw + w * RW][1][lane], f[w], l);
+                probe += state_lds[rw + w * RW][2][lane];
+                some |= state_lds[rw + w * RW][3][lane] != 0.0f;
+            }
+    #pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                if (d % KW != (int)kw) continue;
+    #pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float v = 0.0f;
+    #pragma unroll
+                    for (int w = 0; w < KW; ++w) v = fmaf(sum_at(rw + w * RW, d * 16 + i), f[w], v);
+                    acc[d][i] = v;
                 }
-            } else if constexpr (!PARTS) {
-                store_tile<typename E::A>(static_cast<T *>(a.out) + o0 + 32 * d, acc[d], h);
-            } else if (a.out_dtype == FELLM_DTYPE_F16) {
-                store_tile<F16>(static_cast<_Float16 *>(a.out) + o0 + 32 * d, acc[d], h);
-            } else {
-                store_tile<BF16>(static_cast<uint16_t *>(a.out) + o0 + 32 * d, acc[d], h);
             }
         }
-        if (!direct && h == 0 && kw == 0) {
-            rec[HD] = m;
-            rec[HD + 1] = l;
+
+        // ---- results
+        const bool bad = valid && some && !(probe == 0.0f && l > 0.0f);
+        // exchanges between a row's two lanes follow: both take part or neither, as
+        // valid and bad are the row's
+        if (valid && !bad) {
+            const float inv = !direct ? 1.0f : some ? 1.0f / l : 0.0f;
+            const size_t o0 = (size_t)(t.first + token) * a.out_stride + (size_t)head * HD;
+            float *rec = part + (size_t)(rw * kRows + n) * kRec<HD>;
+    #pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                if (KW > 1 && d % KW != (int)kw) continue;
+    #pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] *= inv;
+                if (!direct || (PARTS && a.out_dtype == FELLM_DTYPE_F32)) {
+                    float *to = direct ? static_cast<float *>(a.out) + o0 : rec;
+    #pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float v[4] = {acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+                        store_f32<F32, 4>(to + 32 * d + 8 * i + 4 * h, v);
+                    }
+                } else if constexpr (!PARTS) {
+                    store_tile<typename E::A>(static_cast<T *>(a.out) + o0 + 32 * d, acc[d], h);
+                } else if (a.out_dtype == FELLM_DTYPE_F16) {
+                    store_tile<F16>(static_cast<_Float16 *>(a.out) + o0 + 32 * d, acc[d], h);
+                } else {
+                    store_tile<BF16>(static_cast<uint16_t *>(a.out) + o0 + 32 * d, acc[d], h);
+                }
+            }
+            if (!direct && h == 0 && kw == 0) {
+                rec[HD] = m;
+                rec[HD + 1] = l;
+            }
         }
-    }
-    uint64_t redo = kw ? 0 : __ballot(bad) & 0xffffffffull;
-    while (redo) {
-        const uint32_t r = (uint32_t)__builtin_ctzll(redo);
-        redo &= redo - 1;
-        const uint32_t pr = t.row0 + rw * kRows + r, tk = a.by_group(pr), hd = g * a.group + pr - tk * a.group;
-        float sums[HD / 64], m1, l1;
-        careful_row<E, HD, PAGED>(a, t, g, tk, hd, sh.begin, sh.end, kBias, sums, m1, l1);
-        const bool none = m1 == -__builtin_inff() && l1 == 0.0f;  // no attended key
-        float *rec = part + (size_t)(rw * kRows + r) * kRec<HD>;
-#pragma unroll
-        for (int e = 0; e < HD / 64; ++e) {
-            if (direct)
-                store_elem(a.out, a.out_dtype, (size_t)(t.first + tk) * a.out_stride + (size_t)hd * HD + lane + 64 * e,
-                           none ? 0.0f : sums[e] / l1);
-            else rec[lane + 64 * e] = sums[e];
+        uint64_t redo = kw ? 0 : __ballot(bad) & 0xffffffffull;
+        while (redo) {
+            const uint32_t r = (uint32_t)__builtin_ctzll(redo);
+            redo &= redo - 1;
+            const uint32_t pr = t.row0 + rw * kRows + r, tk = a.by_group(pr), hd = g * a.group + pr - tk * a.group;
+            float sums[HD / 64], m1, l1;
+            careful_row<E, HD, PAGED>(a, t, g, tk, hd, sh.begin, sh.end, kBias, sums, m1, l1);
+            float *rec = part + (size_t)(rw * kRows + r) * kRec<HD>;
+    #pragma unroll
+            for (int e = 0; e < HD / 64; ++e) {
+                if (direct)
+                    store_elem(a.out, a.out_dtype, (size_t)(t.first + tk) * a.out_stride + (size_t)hd * HD + lane + 64 * e,
+                               sums[e] / l1);
+                else rec[lane + 64 * e] = sums[e];
+            }
+            if (!direct && lane == 0) {
+                rec[HD] = m1;
+                rec[HD + 1] = l1;
+            }
         }
-        if (!direct && lane == 0) {
-            rec[HD] = m1;
-            rec[HD + 1] = l1;
-        }
-    }
     }
 }
 
@@ -959,8 +970,9 @@ __global__ __launch_bounds__(kJoinThreads) void rows_combine(Args a, uint32_t id
     const auto spot = line.template find<true>(id / a.n_kv);
     const Tile t = spot.t;
     if (t.n == 0 || spot.units == 1 || t.row0 + r >= t.n * a.group) return;
-    const uint32_t w0 = spot.at / line.share, w1 = (spot.at + spot.units - 1) / line.share;
-    if (w0 == w1) return;
+    // (offsets that are no offsets could name workgroups that there are none of)
+    const uint32_t w0 = spot.at / line.share, w1 = min((spot.at + spot.units - 1) / line.share, ids - 1);
+    if (w0 >= w1) return;
     // Workgroup w's first record if its piece begins inside the tile or with it, else its second.
     auto record = [&](uint32_t w) {
         const uint32_t slot = 2 * (g * ids + w) + (w * line.share >= spot.at ? 0 : 1);

@@ -3,7 +3,7 @@
 // prefix and the drafted tokens its mask names), or a chunk of a prompt behind
 // a cached prefix (no mask: causal).  The new tokens' K and V are in the cache
 // already, after the prefix.  The kernel is rows_kernel of attention_rows.hpp;
-// long caches of few rows are split over the keys and joined by rows_combine.
+// tiles that several workgroups share are joined by rows_combine.
 #include "attention_rows.hpp"
 
 #include <algorithm>
@@ -22,8 +22,12 @@ struct Layout {
     static constexpr int KT = RW == 4 && HD != 256 && !PARTS ? 64 : 32;
     static constexpr int OCC = HD == 256 || (RW == 1 && HD == 128) ? 1 : 2;
     static constexpr uint32_t BM = kRows * RW, TK = KT * KW;
-    // Workgroups that are resident at once, and the least keys that one takes.
-    static constexpr uint32_t kSlots = 256 * OCC, kMinRounds = (192 + TK - 1) / TK;
+    // Workgroups that are resident at once, and the rounds of the least keys that
+    // one takes, below which the joining costs more than the walk.  Least keys 192,
+    // 128, 64, us: two tokens behind 445 (f32 q, 32/8 heads of 128) 16.4, 14.1,
+    // 14.0; two of 57 behind 330 (64/8) 24.0, 22.6, 27.2; eleven of 21 behind up to
+    // 985 (32/8) 24.7, 26.3, 27.4
+    static constexpr uint32_t kSlots = 256 * OCC, kMinRounds = (128 + TK - 1) / TK;
 };
 
 struct Plan {
@@ -121,7 +125,7 @@ extern "C" int fellm_rocm_paged_tree_attention(const void *q, uint32_t q_dtype, 
     if (n_seqs == 0 || tokens == 0) return FELLM_OK;
     if (!q || !out || !cu_nodes || !prefix_lengths || !kv->arena || !kv->block_table) return FELLM_ERR_ARITY;
     if ((tree_mask != nullptr) != (mask_words != 0) || (tree_mask && window)) return FELLM_ERR_SHAPE;
-    if ((uint64_t)n_kv_heads * head_dim != kv->stride || kv->block_size != rows_attn::kBlockTokens || kv->stride > (1u << 26))
+    if ((uint64_t)n_kv_heads * head_dim != kv->stride || kv->block_size != rows_attn::kBlockTokens || kv->stride > (1u << 25))
         return FELLM_ERR_SHAPE;
     if (kv->block_bytes < 2ull * kv->block_size * kv->stride * 2 || kv->block_bytes % 16) return FELLM_ERR_SHAPE;
     if (kv->layer >= kv->n_layers || kv->n_logical_blocks > (1u << 26)) return FELLM_ERR_SHAPE;

@@ -380,6 +380,7 @@ extern "C" int fellm_rocm_qk_norm_rope(const void *q, uint32_t q_stride, void *q
                                        const float *k_weight, float eps, const float *inv_freqs,
                                        const uint32_t *positions, uint32_t position0, void *stream) {
     using namespace fellm;
+    if (rows == 0) return FELLM_OK;
     if (!q || !q_out || !k || !k_out || !q_weight || !k_weight || (rope_dim && !inv_freqs)) return FELLM_ERR_ARITY;
     NormArgs a{};
     a.q = q, a.k = k, a.q_out = q_out, a.k_out = k_out;
@@ -389,7 +390,6 @@ extern "C" int fellm_rocm_qk_norm_rope(const void *q, uint32_t q_stride, void *q
     a.q_weight = q_weight, a.k_weight = k_weight, a.eps = eps, a.inv_freqs = inv_freqs;
     a.positions = positions, a.position0 = position0;
     if (int rc = check_norm(a)) return rc;
-    if (rows == 0) return FELLM_OK;
     return dispatch_act(act_dtype, [&]<typename A>() -> int { return launch_norm<A, F16, false>(a, as_stream(stream)); });
 }
 
@@ -402,6 +402,7 @@ extern "C" int fellm_rocm_qk_norm_rope_kv_write(const void *q, uint32_t q_stride
                                                 const uint32_t *kv_positions, const uint32_t *sequences,
                                                 const FellmRocmPagedKv *kvp, uint32_t *err_flag, void *stream) {
     using namespace fellm;
+    if (rows == 0) return FELLM_OK;
     if (!q || !q_out || !k || !v || !q_weight || !k_weight || !kv_positions || !kvp || (rope_dim && !inv_freqs))
         return FELLM_ERR_ARITY;
     NormArgs a{};
@@ -415,7 +416,6 @@ extern "C" int fellm_rocm_qk_norm_rope_kv_write(const void *q, uint32_t q_stride
     a.kv_positions = kv_positions, a.sequences = sequences, a.err_flag = err_flag;
     if (!make_kv(kvp, a.kv)) return FELLM_ERR_SHAPE;
     if (int rc = check_norm(a)) return rc;
-    if (rows == 0) return FELLM_OK;
     return dispatch_act(act_dtype, [&]<typename A>() -> int {
         return dispatch_cache(kvp->kv_dtype, [&]<typename C>() -> int { return launch_norm<A, C, true>(a, as_stream(stream)); });
     });

@@ -360,8 +360,9 @@ int fellm_rocm_prompt_attention(const void *q, uint32_t q_stride, const void *k,
  * values than these on the device give right results, more slowly.
  * workspace: fellm_rocm_paged_tree_attention_workspace() bytes, 16-byte
  * aligned, for joining split keys; null or short: no split.  Calls that overlap
- * need a workspace each.  Lengths past the table, and table entries outside the
- * arena, read as zero keys and values.
+ * need a workspace each.  A prefix longer than n_logical_blocks blocks is cut to
+ * them; keys past the table's blocks, and table entries outside the arena, read
+ * as zero keys and values.  out must not overlap q or the cache.
  * As paged decode attention, q and the probabilities are held in 16-bit parts
  * to f32 accuracy when q or out is not of the cache's type; when all three are
  * the same, each is used in that type, the probabilities rounded once.

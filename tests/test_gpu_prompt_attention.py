@@ -150,6 +150,18 @@ def test_attended_infinite_value(ops, dev):
     check(got[..., fine], want[..., fine], tol[..., fine])
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_values_that_all_are_nan(ops, dev, hd):
+    q, k, v, cu = make([300], 4, 2, hd, "bf16", 6)
+    v[:] = float("nan")
+    v[:, 1] = 2.0
+    got = ops.prompt_attention(*(x.to(dev) for x in (q, k, v, cu)), n_heads=4, n_kv_heads=2, head_dim=hd)
+    got = got.view(300, 4, hd)
+    assert torch.isnan(got[:, 2:]).all() and torch.isnan(got[:, :2, 2:]).all()
+    # two: the sums carry n roundings of p and the quotient one of the output
+    assert (got[:, :2, 1] - 2.0).abs().max() <= 2 * (2.0 ** -8 + 300 * 2.0 ** -23)
+
+
 def test_offsets_past_32_bits(ops, dev):
     """Rows 65600 elements apart: the last sequence starts past 4 GiB."""
     stride, t, hd = 65600, 34000, 64

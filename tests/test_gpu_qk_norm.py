@@ -210,6 +210,23 @@ def test_graph(ops, dev):
         assert torch.equal(out, want) and torch.equal(cache.arena, arena)
 
 
+def test_empty(ops, dev):
+    (q, k, v), qw, kw, pos = inputs(4, 4, 2, 64, "f16")
+    q, k, v, qw, kw, pos = (x.to(dev) for x in (q, k, v, qw, kw, pos))
+    got = ops.qk_norm_rope(q[:0], k[:0], qw, kw, 1e-6, inv_freqs(64).to(dev), head_dim=64)
+    assert got[0].shape == (0, 256) and got[1].shape == (0, 128)
+    cache = make_cache(ops, dev, 4, 2, 128, "f16", 8)
+    before = cache.arena.clone()
+    ops.qk_norm_rope_kv_write(q[:0], k[:0], v[:0], qw, kw, 1e-6, inv_freqs(64).to(dev), pos[:0], cache, head_dim=64)
+    assert torch.equal(cache.arena, before)
+
+
+def test_many_rows_of_any_size(ops, dev):
+    """The element-wise kernel and the vector kernel over more workgroups than fit at once."""
+    run_check(ops, dev, 5003, 3, 1, 34, 20, 1, "f32")
+    run_check(ops, dev, 9001, 3, 1, 64, 64, 0, "f32")
+
+
 def test_refusals(ops, dev):
     from fellm_amd import FellmRocmError
 

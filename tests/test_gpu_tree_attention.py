@@ -153,6 +153,46 @@ def test_rows_without_keys_are_zero(ops, dev):
     c.check(got, bits=bits)
 
 
+def test_more_heads_than_a_tile_has_rows(ops, dev):
+    c = Case(ops, dev, [3, 1, 5], [20, 300, 0], 40, 1, 64, "bf16", "bf16")
+    bits = tree_bits(c.nodes)
+    c.check(c.run(ops, bits=bits), bits=bits)
+
+
+@pytest.mark.parametrize("act,kv,hd", [("bf16", "bf16", 128), ("f32", "f16", 64), ("f16", "f16", 256)])
+def test_pieces_that_span_tiles(ops, dev, act, kv, hd):
+    """More tiles than workgroups: each walks several, shared at both ends."""
+    n = 96
+    c = Case(ops, dev, [1 + (7 * i) % 40 for i in range(n)], [(131 * i) % 700 for i in range(n)], 16, 8, hd, act, kv)
+    bits = tree_bits(c.nodes)
+    got = c.run(ops, bits=bits)
+    c.check(got, bits=bits)
+    assert torch.equal(c.run(ops, bits=bits), got)
+
+
+@pytest.mark.parametrize("act,kv,hd,heads", [("bf16", "bf16", 128, 8), ("f16", "f16", 64, 8), ("f32", "bf16", 128, 4)])
+def test_attended_scores_of_minus_infinity(ops, dev, act, kv, hd, heads):
+    """Keys whose scores are -inf weigh nothing, also where they fill a whole share
+    of the keys; a row that has no others is 0 / 0."""
+    n, p = 4, 5000
+    c = Case(ops, dev, [n], [p], heads, 2, hd, act, kv)
+    c.q.view(n, heads, hd)[:, :, 0] = c.q.view(n, heads, hd)[:, :, 0].abs() + 0.25
+    arena = c.cache.arena.view(DT[kv]).view(-1, 2, 16, 2 * hd)
+    blocks = c.cache.block_table.long()[0, 0]
+
+    def hide(first, last):
+        for j in range(first, last):
+            arena[blocks[j // 16], 0, j % 16].view(2, hd)[:, 0] = float("-inf")
+
+    hide(640, 3200)
+    allow = causal_mask(n, p)
+    allow[:, 640:3200] = False
+    want, tol = attend(c.q.view(n, heads, hd), c.k[0], c.v[0], allow, out_dtype=DT[act], **tolerance_args(act, kv, act))
+    check(c.run(ops).view(n, heads, hd), want, tol)
+    hide(0, p + n)
+    assert torch.isnan(c.run(ops)).all()
+
+
 def test_any_mask(ops, dev):
     """Bits above the diagonal, without the token itself, over several words."""
     g = torch.Generator().manual_seed(3)
