@@ -458,44 +458,77 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
 // How a paged launch shares its work.  The rounds of TK keys of every tile, tiles
 // in the order of the sequences, are one line for each K/V head, which the head's
 // `ids` workgroups cut into pieces, so that sequences of any lengths keep every
-// workgroup busy and all of them are resident at once.  Where there are
-// workgroups enough a piece is a part of one tile (per > 1 rounds, share 1);
-// else the line is cut into equal shares, and a workgroup walks the tiles that
-// its share touches, of which the first and the last can be shared with others:
-// two records.  (Measured against tiles cut at fixed numbers of keys: 32 trees of
-// up to 32 tokens behind 616 .. 8192 keys, 64/8 heads of 128, bf16, 124 and 118
-// us; 16 drafted tokens behind 32768 keys, 16/4 heads of 256, 125 and 58.)
+// workgroup busy and all of them are resident at once.
+//  * Where there are workgroups enough a piece is a part of one tile: `per` rounds.
+//  * Else the line is cut into equal shares, and a workgroup walks the tiles that
+//    its share touches, of which the first and the last can be shared with others:
+//    two records.  (Measured against tiles cut at fixed numbers of keys: 32 trees
+//    of up to 32 tokens behind 616 .. 8192 keys, 64/8 heads of 128, bf16, 124 and
+//    118 us; 16 drafted tokens behind 32768 keys, 16/4 heads of 256, 125 and 58.)
+//  * EVEN, for launches of many tiles: every tile begins with
+//    kStart units without keys, what its start costs in rounds, and the tiles of a
+//    causal chunk have rounds that rise with their place in the sequence, tile k
+//    the first one's and k BM / (G TK) more, rounded so that the first k tiles have
+//    floor(k (k - 1) / 2 BM / (G TK)) more than k times the first; the last piece
+//    of a tile takes what is left of its keys.  Shares of it are used where a piece
+//    would be kJoin rounds longer, which is what joining every tile costs.  (8192
+//    tokens behind 8192, 64/8 heads of 128: 4350 -> 3830 us; the 32 trees 118 ->
+//    113.  Its arithmetic costs a launch of few rounds 0.7 of 12 us.)
 // Lane b holds sequence c + b.
-template <uint32_t BM, uint32_t TK>
+template <uint32_t BM, uint32_t TK, bool EVEN>
 struct Line {
+    static constexpr uint32_t kStart = 5, kJoin = 24;
     const Args &a;
     struct Lane {
-        uint32_t first, n, before, tiles, rounds;  // rounds of each tile
+        uint32_t first, n, before, tiles;
     } l0;
-    uint32_t per, share;  // rounds of a unit of the line, units of a workgroup
-    uint32_t units;       // of the line
+    uint32_t per = 1;       // rounds of a unit of the line
+    uint32_t share, units;  // units of a workgroup, of the line
+    uint32_t start = 0;     // units without keys that a tile begins with
+    bool rising = false;
 
-    __device__ __forceinline__ Line(const Args &args, uint32_t ids) : a(args) {
-        l0 = lane(0);
-        per = 1;
+    __device__ __forceinline__ Line(const Args &args, uint32_t ids) : a(args), l0(lane(0)) {
         units = total();
         share = (units + ids - 1) / ids;
-        if (a.part) {
-            per = share = max(share, a.min_rounds);
-            uint32_t pieces = total();
-            if (pieces > ids) {
-                // two rounds more than an equal share cost less than a second
-                // tile's start (about five)
-                per = share + 2;
-                pieces = total();
-            }
-            if (pieces <= ids) share = 1, units = pieces;
-            else per = 1;
+        if (!a.part) return;
+        const uint32_t least = max(share, a.min_rounds);
+        per = least;
+        units = total();
+        if (units > ids) {
+            // two rounds more than an equal share cost less than a second tile's start
+            per = least + 2;
+            units = total();
         }
+        const bool apart = units <= ids;
+        if constexpr (!EVEN) {
+            if (apart) {
+                share = 1;
+            } else {
+                per = 1;
+                units = total();
+                share = least;
+            }
+            return;
+        }
+        const uint32_t parts = units, was = per;
+        rising = !a.mask && !a.window;
+        // (rising rounds are at least half of all)
+        if (!apart || (rising && least / 2 + kJoin < per + kStart)) {
+            per = 1;
+            start = kStart;
+            units = total();
+            share = max((units + ids - 1) / ids, a.min_rounds);
+            if (!apart || share + kJoin < was + kStart) return;
+        }
+        rising = false;
+        per = was;
+        start = 0;
+        units = parts;
+        share = 1;
     }
     __device__ __forceinline__ Lane lane(uint32_t c) const {
         const uint32_t b = c + threadIdx.x % kWave;
-        Lane l{0, 0, 0, 0, 1};
+        Lane l{0, 0, 0, 0};
         if (b < a.n_seqs) {
             l.first = min(a.cu[b], a.tokens);
             const uint32_t end = min(a.cu[b + 1], a.tokens);
@@ -503,51 +536,68 @@ struct Line {
             l.before = min(a.before[b], a.max_before);
         }
         l.tiles = (l.n * a.group + BM - 1) / BM;
-        if (a.part && l.n) {
-            uint32_t keys = l.before + l.n;
-            // the last keys of the tile's first token, its other tokens, the alignment
-            if (a.window) keys = min(keys, min(a.window, 1u << 30) + BM + 63);
-            l.rounds = (keys + TK - 1) / TK;
-        }
         return l;
     }
-    __device__ __forceinline__ uint32_t units_of(const Lane &l) const {
-        return per == 1 ? l.rounds : (l.rounds + per - 1) / per;
+    // Units of the sequence's first tile.
+    __device__ __forceinline__ uint32_t first_units(const Lane &l) const {
+        if (!a.part || !l.n) return 1;
+        uint32_t keys = l.before + (rising ? min(l.n, a.by_group(BM - 1) + 1) : l.n);
+        // the last keys of the tile's first token, its other tokens, the alignment
+        if (a.window) keys = min(keys, min(a.window, 1u << 30) + BM + 63);
+        const uint32_t rounds = (keys + TK - 1) / TK;
+        return per == 1 ? rounds + start : (rounds + per - 1) / per;
+    }
+    // Units of a sequence's first k tiles, u those of the first.
+    __device__ __forceinline__ uint32_t upto(uint32_t u, uint32_t k) const {
+        if (!EVEN || !rising) return k * u;
+        const uint32_t pairs = k ? k * (k - 1) / 2 : 0;
+        return k * u + a.by_group(BM >= TK ? pairs * (BM / TK) : pairs / (TK / BM));
     }
     __device__ __forceinline__ uint32_t total() const {
-        const uint32_t here = l0.tiles * units_of(l0);
+        const uint32_t here = upto(first_units(l0), l0.tiles);
         if (a.n_seqs == 1) return __builtin_amdgcn_readfirstlane(here);
         uint32_t sum = wave_total(here);
         for (uint32_t c = kWave; c < a.n_seqs; c += kWave) {
             const Lane l = lane(c);
-            sum += wave_total(l.tiles * units_of(l));
+            sum += wave_total(upto(first_units(l), l.tiles));
         }
         return sum;
     }
+    // The tile, of `tiles`, that holds unit y of its sequence.
+    __device__ __forceinline__ uint32_t tile_at(uint32_t u, uint32_t tiles, uint32_t y) const {
+        if (!EVEN || !rising) return y / u;
+        // k u + k^2 / 2 step = y to within a tile or two, then exactly
+        const float step = (float)BM / (float)(a.group * TK), b = (float)u - 0.5f * step;
+        const float root = __builtin_amdgcn_sqrtf(fmaf(b, b, 2.0f * step * (float)y));
+        uint32_t k = min(tiles - 1, (uint32_t)fmaxf((root - b) / step, 0.0f));
+        k = __builtin_amdgcn_readfirstlane(k);
+        while (k && upto(u, k) > y) --k;
+        while (k + 1 < tiles && upto(u, k + 1) <= y) ++k;
+        return k;
+    }
     struct Spot {
         Tile t;
-        uint32_t rounds, units, at;  // of the tile, and where it begins on the line
+        uint32_t units, at;  // of the tile, and where it begins on the line
     };
     // BY_TILE: tile number x; else the tile that holds unit x.  n = 0: none.
     template <bool BY_TILE>
     __device__ __forceinline__ Spot find(uint32_t x) const {
-        Spot s{Tile{0, 0, 0, 0, 0}, 1, 1, 0};
+        Spot s{Tile{0, 0, 0, 0, 0}, 1, 0};
         uint32_t tiles = 0, at = 0;
         for (uint32_t c = 0; c < a.n_seqs; c += kWave) {
             const Lane l = c ? lane(c) : l0;
-            const uint32_t u = units_of(l), v = l.tiles * u;
+            const uint32_t u0 = first_units(l), v = upto(u0, l.tiles);
             const bool one = a.n_seqs == 1;
             const uint32_t vi = one ? v : wave_scan(v), ti = !BY_TILE ? 0 : one ? l.tiles : wave_scan(l.tiles);
             const uint64_t past = __ballot((BY_TILE ? tiles + ti : at + vi) > x);
             if (past) {
                 const uint32_t b = (uint32_t)__builtin_ctzll(past);
                 auto of = [&](uint32_t value) { return (uint32_t)__builtin_amdgcn_readlane(value, b); };
-                const uint32_t begin = at + of(vi - v);
-                s.rounds = of(l.rounds);
-                s.units = of(u);
-                const uint32_t k = BY_TILE ? x - (tiles + of(ti - l.tiles)) : (x - begin) / s.units;
+                const uint32_t begin = at + of(vi - v), u = of(u0);
+                const uint32_t k = BY_TILE ? x - (tiles + of(ti - l.tiles)) : tile_at(u, of(l.tiles), x - begin);
                 s.t = Tile{c + b, k * BM, of(l.first), of(l.n), of(l.before)};
-                s.at = begin + k * s.units;
+                s.at = begin + upto(u, k);
+                s.units = upto(u, k + 1) - upto(u, k);
                 return s;
             }
             if (BY_TILE) tiles += __builtin_amdgcn_readlane(ti, kWave - 1);
@@ -574,7 +624,7 @@ __device__ __forceinline__ Rsrc uniform_rsrc(const uint8_t *p, uint32_t range) {
 // 16-bit parts (q or out in f32, or q of another 16-bit type than K/V).
 // OCC: wavefronts per SIMD the registers are kept for.  (Three tiles in LDS
 // instead of two, two of them on their way, measured the same within 1%.)
-template <typename E, int HD, int RW, int KW, int KT, bool PAGED, bool PARTS, int OCC>
+template <typename E, int HD, int RW, int KW, int KT, bool PAGED, bool PARTS, int OCC, bool EVEN = false>
 __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     constexpr int NW = RW * KW, NS = HD / 16, NU = KT / 32, ND = HD / 32;
     constexpr int QP = PARTS ? E::kQParts : 1, PP = PARTS ? E::kPParts : 1;
@@ -597,7 +647,7 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
     const uint32_t g = blockIdx.x % a.n_kv, id = blockIdx.x / a.n_kv, ids = gridDim.x / a.n_kv;
     // this workgroup's piece [x, x_end) of the line (contiguous K/V: its one tile)
     const auto line = [&] {
-        if constexpr (PAGED) return Line<BM, TK>(a, ids);
+        if constexpr (PAGED) return Line<BM, TK, EVEN>(a, ids);
         else return 0;
     }();
     uint32_t x = 0, x_end = 1;
@@ -617,14 +667,15 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
             if (t.n == 0) break;  // offsets that are none: nothing more to find
             sh = tile_keys<BM>(a, t);
             const uint32_t u0 = x - spot.at, u1 = min(spot.units, u0 + x_end - x);
-            direct = u1 - u0 == spot.units;
+            x += u1 - u0;
+            if (u1 <= line.start) break;  // the share ends before the tile's keys
+            direct = u0 <= line.start && u1 == spot.units;
             if (!direct) {
                 part = a.part + (size_t)(2 * (g * ids + id) + again) * BM * kRec<HD>;
                 const uint32_t lo = sh.begin;
-                sh.begin = lo + u0 * line.per * TK;
-                if (u1 < spot.units) sh.end = min(sh.end, lo + u1 * line.per * TK);
+                if (u0 > line.start) sh.begin = lo + (u0 - line.start) * line.per * TK;
+                if (u1 < spot.units) sh.end = min(sh.end, lo + (u1 - line.start) * line.per * TK);
             }
-            x += u1 - u0;
             if (again) __syncthreads();  // the buffers may still be read for the tile before
         } else {
             t = tile_of<BM>(a, id, ids);
@@ -960,18 +1011,18 @@ __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
 // one record, Q groups of 16 lanes every Q-th.  ids: the workgroups per K/V head
 // of the launch before.
 constexpr uint32_t kJoinThreads = 256;
-template <int HD, uint32_t BM, uint32_t TK, int Q>
+template <int HD, uint32_t BM, uint32_t TK, int Q, bool EVEN>
 __global__ __launch_bounds__(kJoinThreads) void rows_combine(Args a, uint32_t ids) {
     constexpr uint32_t ROWS = kJoinThreads / 16 / Q;  // of a workgroup
     const uint32_t id = blockIdx.x / (BM / ROWS), g = id % a.n_kv;
     const uint32_t r = blockIdx.x % (BM / ROWS) * ROWS + threadIdx.x / (16 * Q);
     const uint32_t col = threadIdx.x % 16, part = threadIdx.x / 16 % Q;
-    const Line<BM, TK> line(a, ids);
+    const Line<BM, TK, EVEN> line(a, ids);
     const auto spot = line.template find<true>(id / a.n_kv);
     const Tile t = spot.t;
     if (t.n == 0 || spot.units == 1 || t.row0 + r >= t.n * a.group) return;
     // (offsets that are no offsets could name workgroups that there are none of)
-    const uint32_t w0 = spot.at / line.share, w1 = min((spot.at + spot.units - 1) / line.share, ids - 1);
+    const uint32_t w0 = (spot.at + line.start) / line.share, w1 = min((spot.at + spot.units - 1) / line.share, ids - 1);
     if (w0 >= w1) return;
     // Workgroup w's first record if its piece begins inside the tile or with it, else its second.
     auto record = [&](uint32_t w) {

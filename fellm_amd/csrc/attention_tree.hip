@@ -66,7 +66,7 @@ auto with_layout(uint32_t head_dim, uint64_t rows, bool parts, Fn &&f) {
     return parts ? pick_head.template operator()<true>() : pick_head.template operator()<false>();
 }
 
-template <typename E, int HD, int RW, bool PARTS>
+template <typename E, int HD, int RW, bool PARTS, bool EVEN>
 int launch_tree(const Plan &p, Args a, hipStream_t st) {
     using L = Layout<HD, RW, PARTS>;
     const uint64_t grid = (uint64_t)p.ids * a.n_kv, rows = p.tiles * a.n_kv * L::BM;
@@ -74,14 +74,14 @@ int launch_tree(const Plan &p, Args a, hipStream_t st) {
     if (std::max(grid * 4 * kWave, rows * 64) > 0xffffffffull) return FELLM_ERR_SHAPE;
     if (p.tiles * (((uint64_t)a.max_before + a.tokens) / L::TK + 1) > 0x3fffffffull) return FELLM_ERR_SHAPE;
     a.min_rounds = L::kMinRounds;
-    FELLM_LAUNCH((rows_kernel<E, HD, RW, L::KW, L::KT, true, PARTS, L::OCC>), dim3((uint32_t)grid),
+    FELLM_LAUNCH((rows_kernel<E, HD, RW, L::KW, L::KT, true, PARTS, L::OCC, EVEN>), dim3((uint32_t)grid),
                  dim3(kWave * RW * L::KW), 0, st, a);
     int rc = launch_status();
     if (rc != FELLM_OK || !a.part) return rc;
     // 64 lanes a row where a tile can have many records (one sequence of 32768
     // keys, 28/4 heads: 44.0 -> 38.1 us; eight of up to 1000 the other way 22.5, 24.6)
     auto join = [&]<int Q>() {
-        FELLM_LAUNCH((rows_combine<HD, L::BM, L::TK, Q>), dim3((uint32_t)(rows / (kJoinThreads / 16 / Q))),
+        FELLM_LAUNCH((rows_combine<HD, L::BM, L::TK, Q, EVEN>), dim3((uint32_t)(rows / (kJoinThreads / 16 / Q))),
                      dim3(kJoinThreads), 0, st, a, p.ids);
     };
     if (p.ids > 4 * p.tiles) join.template operator()<4>();
@@ -169,7 +169,15 @@ extern "C" int fellm_rocm_paged_tree_attention(const void *q, uint32_t q_dtype, 
     return with_layout(head_dim, (uint64_t)nodes * a.group, parts, [&]<int HD, int RW, bool PARTS>() {
         const Plan p = plan<HD, RW, PARTS>(n_seqs, tokens, a.group, n_kv_heads, nodes, max_prefix);
         a.part = p.part_bytes && workspace && workspace_bytes >= p.part_bytes ? workspace : nullptr;
-        return kv->kv_dtype == FELLM_DTYPE_BF16 ? launch_tree<rows_attn::ElemBF16, HD, RW, PARTS>(p, a, st)
-                                                : launch_tree<rows_attn::ElemF16, HD, RW, PARTS>(p, a, st);
+        auto launch = [&]<bool EVEN>() {
+            return kv->kv_dtype == FELLM_DTYPE_BF16 ? launch_tree<rows_attn::ElemBF16, HD, RW, PARTS, EVEN>(p, a, st)
+                                                    : launch_tree<rows_attn::ElemF16, HD, RW, PARTS, EVEN>(p, a, st);
+        };
+        // rows for at least a tile to three workgroups, which ragged trees double
+        // (and below 32768 tiles: the sums of Line::upto stay below 2^32)
+        const uint64_t whole = (uint64_t)tokens * a.group / (rows_attn::kRows * RW);
+        if constexpr (RW == 4)
+            if (a.part && 3 * whole >= p.ids && whole < 32768) return launch.template operator()<true>();
+        return launch.template operator()<false>();
     });
 }

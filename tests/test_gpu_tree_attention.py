@@ -170,6 +170,17 @@ def test_pieces_that_span_tiles(ops, dev, act, kv, hd):
     assert torch.equal(c.run(ops, bits=bits), got)
 
 
+@pytest.mark.parametrize("nodes,prefix,heads,kv_heads,hd", [
+    ([2100], [0], 24, 4, 64), ([1500, 1, 0, 700], [0, 50, 9, 333], 16, 2, 128), ([1030], [600], 7, 1, 256),
+    ([9] * 70, [40] * 70, 64, 8, 64)])
+def test_long_chunks(ops, dev, nodes, prefix, heads, kv_heads, hd):
+    """Causal chunks whose tiles have rising numbers of keys, in shares of equal work."""
+    c = Case(ops, dev, nodes, prefix, heads, kv_heads, hd, "bf16", "bf16")
+    got = c.run(ops)
+    c.check(got)
+    assert torch.equal(c.run(ops), got)
+
+
 @pytest.mark.parametrize("act,kv,hd,heads", [("bf16", "bf16", 128, 8), ("f16", "f16", 64, 8), ("f32", "bf16", 128, 4)])
 def test_attended_scores_of_minus_infinity(ops, dev, act, kv, hd, heads):
     """Keys whose scores are -inf weigh nothing, also where they fill a whole share
