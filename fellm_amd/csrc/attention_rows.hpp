@@ -622,7 +622,7 @@ __device__ __forceinline__ Rsrc uniform_rsrc(const uint8_t *p, uint32_t range) {
 // wavefronts that share those rows and take every KW-th key tile, KT: keys of
 // a wavefront's tile (32 or 64), PARTS: q and p held to f32 accuracy in several
 // 16-bit parts (q or out in f32, or q of another 16-bit type than K/V).
-// OCC: wavefronts per SIMD the registers are kept for.  (Three tiles in LDS
+// OCC: wavefronts per SIMD the registers are kept for.  EVEN: see Line.  (Three tiles in LDS
 // instead of two, two of them on their way, measured the same within 1%.)
 template <typename E, int HD, int RW, int KW, int KT, bool PAGED, bool PARTS, int OCC, bool EVEN = false>
 __global__ __launch_bounds__(kWave *RW *KW, OCC) void rows_kernel(Args a) {
