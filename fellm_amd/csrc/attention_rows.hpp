@@ -472,7 +472,7 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
 //    floor(k (k - 1) / 2 BM / (G TK)) more than k times the first; the last piece
 //    of a tile takes what is left of its keys.  Shares of it are used where a piece
 //    would be kJoin rounds longer, which is what joining every tile costs.  (8192
-//    tokens behind 8192, 64/8 heads of 128: 4350 -> 3830 us; the 32 trees 118 ->
+//    tokens behind 8192, 64/8 heads of 128: 4610 -> 3940 us; the 32 trees 118 ->
 //    113.  Its arithmetic costs a launch of few rounds 0.7 of 12 us.)
 // Lane b holds sequence c + b.
 template <uint32_t BM, uint32_t TK, bool EVEN>
